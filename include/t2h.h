@@ -205,6 +205,101 @@ int32_t t2h_attn_pack(const void* q, const void* k, const void* v,
                       int64_t mp, void* k_out, void* vh, int64_t lp,
                       int32_t k_transposed, void* stream);
 
+/* ---- attention -----------------------------------------------------------------
+ * out_i = sum_j exp(s_ij - lse_i) v_j,  s_ij = scale * q_i . k_j,
+ * lse_i = log sum_j exp(s_ij), j over the keys of row i's segment.
+ * Replaces the chain's scores GEMM, softmax_rows_z and output GEMM between
+ * the packs and unpack_o_z (gpu/attention.mojo:77-331, 566-689), and the
+ * varlen attention of sparse/attention/full_attn.mojo, in one pass over the
+ * keys on the matrix cores: no scores in memory.
+ * q, out [q_rows, heads, head_dim], k, v [k_rows, kv_heads, head_dim], f16 or
+ * bf16, head_dim 64 or 128; heads a multiple of kv_heads (query head h reads
+ * key/value head h / (heads / kv_heads)). Sums and softmax in f32; the
+ * exponentials are rounded to dtype for the product with v.
+ * strides_host: (row, head) strides in elements of q, k, v, out (8 values; 0 =
+ * contiguous), so that the operands can be views of a packed qkv [rows, 3, H,
+ * D] (row 3HD, head D) or the head-major outputs of t2h_attn_pack /
+ * t2h_qkv_linear_pack (row D, head mp * D; qh holds the scale: pass 1); NULL =
+ * all contiguous. Multiples of 8, rows at most 2^23; 16-byte aligned tensors.
+ * Segments: nbatch of them, rows [offsets[b], offsets[b + 1]) (int64 device
+ * [nbatch + 1]) or equal shares where a side's offsets are NULL. k_lens (int64
+ * device [nbatch] or NULL): only that many keys at the start of a segment
+ * count; what lies in the others is not used, whatever it is. A row without
+ * keys gets out 0 and lse -inf. Rows outside the segments are not written.
+ * lse [heads, q_rows] f32 or NULL. out must not overlap the inputs.
+ * workspace: t2h_attention_workspace() bytes (16-byte aligned, any contents)
+ * let calls of few rows split their keys over the GPU; with less, or NULL,
+ * they run unsplit (same result up to rounding, more time). Calls that
+ * share a workspace must not overlap. Repeated calls give the same bits. */
+int64_t t2h_attention_workspace(int64_t q_rows, int64_t k_rows, int32_t heads,
+                                int32_t kv_heads, int32_t head_dim,
+                                int32_t nbatch);
+int32_t t2h_attention(const void* q, const void* k, const void* v, void* out,
+                      float* lse, const int64_t* strides_host, int64_t q_rows,
+                      int64_t k_rows, int32_t heads, int32_t kv_heads,
+                      int32_t head_dim, int32_t dtype, float scale,
+                      const int64_t* q_offsets, const int64_t* k_offsets,
+                      const int64_t* k_lens, int32_t nbatch, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* Backward pass of t2h_attention (no counterpart in the reference, which only
+ * infers): from dout, the forward's operands, its out and its lse
+ *   P_ij = exp(s_ij - lse_i), delta_i = sum_d dout_id out_id,
+ *   dS_ij = P_ij (dout_i . v_j - delta_i),
+ *   dv_j = sum_i P_ij dout_i, dq_i = scale sum_j dS_ij k_j,
+ *   dk_j = scale sum_i dS_ij q_i,
+ * with dk and dv summed over the query heads of a key/value head. P and dS are
+ * rounded to dtype for the products, sums are f32. Shapes and segments as
+ * t2h_attention; strides_host: 16 values, of q, k, v, out, dout, dq, dk, dv.
+ * Keys that do not count get dk = dv = 0, rows without keys dq = 0; rows
+ * outside the segments are not written. The gradients must not overlap the
+ * inputs or each other (they may be views of one packed buffer). workspace:
+ * t2h_attention_backward_workspace() bytes, required. No atomic sums:
+ * repeated calls give the same bits. */
+int64_t t2h_attention_backward_workspace(int64_t q_rows, int64_t k_rows,
+                                         int32_t heads, int32_t kv_heads,
+                                         int32_t head_dim, int32_t nbatch);
+int32_t t2h_attention_backward(const void* q, const void* k, const void* v,
+                               const void* out, const float* lse,
+                               const void* dout, void* dq, void* dk, void* dv,
+                               const int64_t* strides_host, int64_t q_rows,
+                               int64_t k_rows, int32_t heads, int32_t kv_heads,
+                               int32_t head_dim, int32_t dtype, float scale,
+                               const int64_t* q_offsets,
+                               const int64_t* k_offsets, const int64_t* k_lens,
+                               int32_t nbatch, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/* Backward pass of t2h_qk_rmsnorm_rope (no counterpart in the reference): with
+ * x = in + bias, n = max(|x|, 1e-12), xh = x / n per head, R the rotation
+ * and g = R^T dout:
+ *   w = g * gamma * sqrt(head_dim), din = (w - xh (xh . w)) / n
+ *   (n at its floor: din = w / n; no gammas: din = g),
+ *   dgamma = sqrt(head_dim) sum_rows g * xh, dbias = sum_rows din.
+ * q_in / k_in: the forward's inputs (row stride in_stride; read only for a
+ * norm), dq_out / dk_out the gradients of its outputs (dout_stride), dq_in /
+ * dk_in those of its inputs (din_stride; in place on dq_out / dk_out with
+ * equal strides). Either of q and k may be NULL throughout. Parameters and
+ * positions as in t2h_qk_rmsnorm_rope; gamma_q without gamma_k is allowed.
+ * dgamma_*, dbias_* [heads, head_dim] f32, overwritten, or NULL; any of them
+ * needs a workspace of t2h_qk_rmsnorm_rope_backward_workspace() bytes
+ * (tensors: how many of q and k are given). The sums are f32, in a fixed
+ * order. */
+int64_t t2h_qk_rmsnorm_rope_backward_workspace(int64_t rows, int32_t heads,
+                                               int32_t head_dim,
+                                               int32_t tensors);
+int32_t t2h_qk_rmsnorm_rope_backward(
+    const void* q_in, const void* k_in, const void* dq_out, const void* dk_out,
+    void* dq_in, void* dk_in, int64_t rows, int64_t in_stride,
+    int64_t dout_stride, int64_t din_stride, int32_t heads, int32_t head_dim,
+    int32_t dtype, const float* bias_q, const float* bias_k,
+    const float* gamma_q, const float* gamma_k, int32_t use_rope,
+    const float* freqs_host, int32_t freq_dim, int32_t pos_dim,
+    const float* phases, int64_t phase_rows, const int32_t* coords,
+    int32_t coord_cols, int32_t grid_res, float* dgamma_q, float* dgamma_k,
+    float* dbias_q, float* dbias_k, void* workspace, int64_t workspace_bytes,
+    void* stream);
+
 /* ---- linear fused with the gated residual join ------------------------------
  * out[t, n] = res[t, n] + fl(fl(sum_k x[t, k] * w[n, k] + bias[n]) * gate[b(t), n])
  * (gate NULL: res + fl(acc + bias)): the block's residual join in the store

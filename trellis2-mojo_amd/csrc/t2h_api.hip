@@ -17,6 +17,7 @@
 #include "t2h.h"
 #include <cstdlib>
 
+#include "t2h_attn.h"
 #include "t2h_internal.h"
 
 namespace t2h {
@@ -425,6 +426,241 @@ int32_t t2h_attn_pack(const void* q, const void* k, const void* v, int64_t in_st
     a.lp = lp;
     a.k_transposed = k_transposed ? 1 : 0;
     return hip_status(launch_pack(a, tab, static_cast<hipStream_t>(stream)), fn);
+}
+
+int64_t t2h_qk_rmsnorm_rope_backward_workspace(int64_t rows, int32_t heads, int32_t head_dim, int32_t tensors) {
+    if (rows < 0 || heads <= 0 || head_dim <= 0 || tensors < 1 || tensors > 2) return -1;
+    return qk_bwd_bytes(rows, heads, head_dim, tensors);
+}
+
+int32_t t2h_qk_rmsnorm_rope_backward(const void* q_in, const void* k_in, const void* dq_out, const void* dk_out,
+                                     void* dq_in, void* dk_in, int64_t rows, int64_t in_stride, int64_t dout_stride,
+                                     int64_t din_stride, int32_t heads, int32_t head_dim, int32_t dtype,
+                                     const float* bias_q, const float* bias_k, const float* gamma_q,
+                                     const float* gamma_k, int32_t use_rope, const float* freqs_host, int32_t freq_dim,
+                                     int32_t pos_dim, const float* phases, int64_t phase_rows, const int32_t* coords,
+                                     int32_t coord_cols, int32_t grid_res, float* dgamma_q, float* dgamma_k,
+                                     float* dbias_q, float* dbias_k, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+    const char* fn = "t2h_qk_rmsnorm_rope_backward";
+    if (!dtype_ok(dtype)) return fail(T2H_EINVAL, "%s: bad dtype %d", fn, dtype);
+    if (rows < 0 || heads <= 0 || heads > 65535 || head_dim <= 0 || head_dim % 2 != 0)
+        return fail(T2H_EINVAL, "%s: bad shape", fn);
+    if (head_dim > 2 * T2H_MAX_HALF_HEAD) return fail(T2H_EUNSUPPORTED, "%s: head_dim > %d", fn, 2 * T2H_MAX_HALF_HEAD);
+    const int64_t hd = (int64_t)heads * head_dim;
+    if (in_stride == 0) in_stride = hd;
+    if (dout_stride == 0) dout_stride = hd;
+    if (din_stride == 0) din_stride = hd;
+    if (in_stride < hd || dout_stride < hd || din_stride < hd)
+        return fail(T2H_EINVAL, "%s: row stride < heads * head_dim", fn);
+    RopeSlots tab;
+    std::memset(&tab, 0, sizeof(tab));
+    if (use_rope) {
+        if (int32_t rc = build_slots(head_dim, freqs_host, freq_dim, pos_dim, tab, fn)) return rc;
+        if (int32_t rc = check_positions(phases, phase_rows, coords, coord_cols, grid_res, pos_dim, fn)) return rc;
+    }
+    QkBwdArgs a{};
+    const QkBwdTensor both[2] = {{q_in, dq_out, dq_in, bias_q, gamma_q, dgamma_q, dbias_q},
+                                 {k_in, dk_out, dk_in, bias_k, gamma_k, dgamma_k, dbias_k}};
+    bool sums = false;
+    for (int i = 0; i < 2; ++i) {
+        const QkBwdTensor& t = both[i];
+        if (t.dy == nullptr && t.dx == nullptr) {
+            if (t.dgamma == nullptr && t.dbias == nullptr) continue;
+            if (rows > 0) return fail(T2H_EINVAL, "%s: a parameter's gradient needs its tensor's", fn);
+        }
+        if (rows > 0 && (t.dy == nullptr || t.dx == nullptr)) return fail(T2H_EINVAL, "%s: NULL tensor", fn);
+        if (rows > 0 && t.gamma != nullptr && t.x == nullptr) return fail(T2H_EINVAL, "%s: the norm's gradient needs its input", fn);
+        if (t.gamma == nullptr && t.dgamma != nullptr) return fail(T2H_EINVAL, "%s: dgamma without gamma", fn);
+        if (t.dx == t.x && t.x != nullptr && t.gamma != nullptr && din_stride != in_stride)
+            return fail(T2H_EINVAL, "%s: in place needs equal row strides", fn);
+        if (t.dx == t.dy && t.dx != nullptr && din_stride != dout_stride) return fail(T2H_EINVAL, "%s: in place needs equal row strides", fn);
+        sums = sums || t.dgamma != nullptr || t.dbias != nullptr;
+        a.t[a.tensors++] = t;
+    }
+    if (a.tensors == 0 && rows > 0) return fail(T2H_EINVAL, "%s: dq and dk are both NULL", fn);
+    if (a.tensors == 0) return ok();
+    if (sums && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < qk_bwd_bytes(rows, heads, head_dim, a.tensors)))
+        return fail(T2H_EINVAL, "%s: needs a workspace of %lld bytes (16-byte aligned)", fn,
+                    (long long)qk_bwd_bytes(rows, heads, head_dim, a.tensors));
+    if (!sums) workspace = nullptr;
+    if (rows == 0 && !sums) return ok();
+    a.rows = rows;
+    a.x_stride = in_stride;
+    a.dy_stride = dout_stride;
+    a.dx_stride = din_stride;
+    a.heads = heads;
+    a.head_dim = head_dim;
+    a.dtype = dtype;
+    a.rms_scale = (float)std::sqrt((double)head_dim);
+    a.use_rope = use_rope ? 1 : 0;
+    a.pos_dim = pos_dim;
+    a.freq_dim = freq_dim;
+    a.phases = use_rope ? phases : nullptr;
+    a.phase_rows = phase_rows;
+    a.coords = (use_rope && phases == nullptr) ? coords : nullptr;
+    a.coord_cols = coord_cols;
+    a.grid_res = grid_res;
+    a.part = static_cast<float*>(workspace);
+    return hip_status(launch_qk_bwd(a, tab, static_cast<hipStream_t>(stream)), fn);
+}
+
+}  // extern "C"
+
+// ---- attention ----------------------------------------------------------------
+namespace t2h {
+namespace {
+
+// Row strides reach 64 rows on in 32-bit byte offsets.
+constexpr int64_t kAttnMaxRowStride = int64_t(1) << 23;
+
+int32_t attn_sizes(const char* fn, int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                   int32_t nbatch) {
+    if (q_rows < 0 || k_rows < 0 || heads <= 0 || heads > 65535 || kv_heads <= 0)
+        return fail(T2H_EINVAL, "%s: bad shape", fn);
+    if (heads % kv_heads != 0) return fail(T2H_EINVAL, "%s: heads must be a multiple of kv_heads", fn);
+    if (head_dim != 64 && head_dim != 128) return fail(T2H_EUNSUPPORTED, "%s: head_dim must be 64 or 128", fn);
+    if (nbatch < 1) return fail(T2H_EINVAL, "%s: nbatch < 1", fn);
+    if (q_rows > INT32_MAX || k_rows > INT32_MAX) return fail(T2H_EUNSUPPORTED, "%s: more than 2^31 - 1 rows", fn);
+    // block numbers are 32-bit, with up to 64 parts of each tile
+    if ((q_rows / 64 + nbatch) * heads >= INT32_MAX / 64 || (k_rows / 64 + nbatch) * kv_heads >= INT32_MAX / 64)
+        return fail(T2H_EUNSUPPORTED, "%s: too many tiles", fn);
+    return T2H_OK;
+}
+
+// One tensor's strides (0 = contiguous [rows, heads, head_dim]) and alignment.
+int32_t attn_tensor(const char* fn, const char* name, const void* p, int64_t rows, int32_t heads, int32_t head_dim,
+                    const int64_t* strides_host, int i, int64_t& row, int64_t& head) {
+    row = strides_host != nullptr ? strides_host[2 * i] : 0;
+    head = strides_host != nullptr ? strides_host[2 * i + 1] : 0;
+    if (row == 0) row = (int64_t)heads * head_dim;
+    if (head == 0) head = head_dim;
+    if (rows > 0 && p == nullptr) return fail(T2H_EINVAL, "%s: %s is NULL", fn, name);
+    if (row < head_dim || head < head_dim || row % 8 != 0 || head % 8 != 0)
+        return fail(T2H_EINVAL, "%s: %s strides must be multiples of 8 elements, at least head_dim", fn, name);
+    if (row > kAttnMaxRowStride) return fail(T2H_EUNSUPPORTED, "%s: %s row stride above 2^23 elements", fn, name);
+    if (!aligned(p, 16)) return fail(T2H_EINVAL, "%s: %s must be 16-byte aligned", fn, name);
+    return T2H_OK;
+}
+
+int32_t attn_common(const char* fn, AttnArgs& a, const void* q, const void* k, const void* v, const void* out,
+                    const int64_t* strides_host, int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads,
+                    int32_t head_dim, int32_t dtype, float scale, const int64_t* q_offsets, const int64_t* k_offsets,
+                    const int64_t* k_lens, int32_t nbatch) {
+    if (dtype != T2H_F16 && dtype != T2H_BF16)
+        return fail(dtype == T2H_F32 ? T2H_EUNSUPPORTED : T2H_EINVAL, "%s: dtype must be f16 or bf16", fn);
+    if (int32_t rc = attn_sizes(fn, q_rows, k_rows, heads, kv_heads, head_dim, nbatch)) return rc;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(T2H_EINVAL, "%s: scale must be positive and finite", fn);
+    if ((q_offsets == nullptr && q_rows % nbatch != 0) || (k_offsets == nullptr && k_rows % nbatch != 0))
+        return fail(T2H_EINVAL, "%s: rows without offsets must divide into nbatch segments", fn);
+    if (int32_t rc = attn_tensor(fn, "q", q, q_rows, heads, head_dim, strides_host, 0, a.q_row, a.q_head)) return rc;
+    if (int32_t rc = attn_tensor(fn, "k", k, k_rows, kv_heads, head_dim, strides_host, 1, a.k_row, a.k_head)) return rc;
+    if (int32_t rc = attn_tensor(fn, "v", v, k_rows, kv_heads, head_dim, strides_host, 2, a.v_row, a.v_head)) return rc;
+    if (int32_t rc = attn_tensor(fn, "out", out, q_rows, heads, head_dim, strides_host, 3, a.o_row, a.o_head)) return rc;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = const_cast<void*>(out);
+    a.q_rows = q_rows;
+    a.k_rows = k_rows;
+    a.heads = heads;
+    a.group = heads / kv_heads;
+    a.head_dim = head_dim;
+    a.dtype = dtype;
+    a.scale = scale;
+    a.q_offsets = q_offsets;
+    a.k_offsets = k_offsets;
+    a.k_lens = k_lens;
+    a.nbatch = nbatch;
+    return T2H_OK;
+}
+
+}  // namespace
+}  // namespace t2h
+
+extern "C" {
+
+int64_t t2h_attention_workspace(int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                int32_t nbatch) {
+    if (attn_sizes("t2h_attention_workspace", q_rows, k_rows, heads, kv_heads, head_dim, nbatch) != T2H_OK) return -1;
+    AttnArgs a{};
+    a.q_rows = q_rows;
+    a.k_rows = k_rows;
+    a.heads = heads;
+    a.group = heads / kv_heads;
+    a.head_dim = head_dim;
+    a.nbatch = nbatch;
+    return attn_split_bytes(a, attn_splits(a));
+}
+
+int32_t t2h_attention(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t* strides_host,
+                      int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype,
+                      float scale, const int64_t* q_offsets, const int64_t* k_offsets, const int64_t* k_lens,
+                      int32_t nbatch, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* fn = "t2h_attention";
+    AttnArgs a{};
+    if (int32_t rc = attn_common(fn, a, q, k, v, out, strides_host, q_rows, k_rows, heads, kv_heads, head_dim, dtype,
+                                 scale, q_offsets, k_offsets, k_lens, nbatch))
+        return rc;
+    if (q_rows == 0) return ok();
+    if (out == q || out == k || out == v) return fail(T2H_EINVAL, "%s: out must not alias an input", fn);
+    if (!aligned(workspace, 16)) return fail(T2H_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+    a.lse = lse;
+    a.nsplit = attn_splits(a);
+    const int64_t need = attn_split_bytes(a, a.nsplit);
+    if (workspace == nullptr || workspace_bytes < need) a.nsplit = 1;
+    if (a.nsplit > 1) {
+        a.part = static_cast<float*>(workspace);
+        a.part_lse = a.part + (int64_t)a.nsplit * q_rows * heads * head_dim;
+    }
+    return hip_status(launch_attn(a, static_cast<hipStream_t>(stream)), fn);
+}
+
+int64_t t2h_attention_backward_workspace(int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads,
+                                         int32_t head_dim, int32_t nbatch) {
+    if (attn_sizes("t2h_attention_backward_workspace", q_rows, k_rows, heads, kv_heads, head_dim, nbatch) != T2H_OK)
+        return -1;
+    AttnBwdArgs a{};
+    a.f.q_rows = q_rows;
+    a.f.k_rows = k_rows;
+    a.f.heads = heads;
+    a.f.group = heads / kv_heads;
+    a.f.head_dim = head_dim;
+    a.f.nbatch = nbatch;
+    a.kv_heads = kv_heads;
+    return attn_bwd_plan(a, nullptr);
+}
+
+int32_t t2h_attention_backward(const void* q, const void* k, const void* v, const void* out, const float* lse,
+                               const void* dout, void* dq, void* dk, void* dv, const int64_t* strides_host,
+                               int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                               int32_t dtype, float scale, const int64_t* q_offsets, const int64_t* k_offsets,
+                               const int64_t* k_lens, int32_t nbatch, void* workspace, int64_t workspace_bytes,
+                               void* stream) {
+    const char* fn = "t2h_attention_backward";
+    AttnBwdArgs a{};
+    if (int32_t rc = attn_common(fn, a.f, q, k, v, out, strides_host, q_rows, k_rows, heads, kv_heads, head_dim, dtype,
+                                 scale, q_offsets, k_offsets, k_lens, nbatch))
+        return rc;
+    if (int32_t rc = attn_tensor(fn, "dout", dout, q_rows, heads, head_dim, strides_host, 4, a.do_row, a.do_head)) return rc;
+    if (int32_t rc = attn_tensor(fn, "dq", dq, q_rows, heads, head_dim, strides_host, 5, a.dq_row, a.dq_head)) return rc;
+    if (int32_t rc = attn_tensor(fn, "dk", dk, k_rows, kv_heads, head_dim, strides_host, 6, a.dk_row, a.dk_head)) return rc;
+    if (int32_t rc = attn_tensor(fn, "dv", dv, k_rows, kv_heads, head_dim, strides_host, 7, a.dv_row, a.dv_head)) return rc;
+    if (q_rows == 0 && k_rows == 0) return ok();
+    if (q_rows > 0 && lse == nullptr) return fail(T2H_EINVAL, "%s: lse is NULL", fn);
+    const void* in[5] = {q, k, v, out, dout};
+    for (const void* p : in)
+        if (p != nullptr && (p == dq || p == dk || p == dv)) return fail(T2H_EINVAL, "%s: gradients must not alias inputs", fn);
+    a.kv_heads = kv_heads;
+    const int64_t need = attn_bwd_plan(a, workspace);
+    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need)
+        return fail(T2H_EINVAL, "%s: needs a workspace of %lld bytes (16-byte aligned)", fn, (long long)need);
+    a.dout = dout;
+    a.dq = dq;
+    a.dk = dk;
+    a.dv = dv;
+    a.f.lse = const_cast<float*>(lse);
+    return hip_status(launch_attn_bwd(a, static_cast<hipStream_t>(stream)), fn);
 }
 
 int32_t t2h_qkv_linear_pack(const void* x, int64_t ldx, const void* w, int64_t rows, int32_t in_features,

@@ -1,0 +1,605 @@
+// Backward pass of the attention (t2h_attn.hip), with the probabilities
+// computed again from the operands and the forward's log-sum-exp:
+//
+//   P_ij = exp(scale q_i.k_j - lse_i)      delta_i = sum_d dout_id out_id
+//   dP_ij = dout_i.v_j                     dS_ij = P_ij (dP_ij - delta_i)
+//   dv_j = sum_i P_ij dout_i    dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i
+//
+// Three launches: delta (and, for f16, the largest row lengths); dk and dv with
+// the keys kept in registers and the queries streaming; dq with the queries
+// kept and the keys streaming. The last two compute P and dP twice, seven
+// products in place of five, and need no atomic sums, whose order would change
+// the result from run to run.
+//
+// f16: P is rounded as 2^14 P (P is near 1 / keys, below f16's smallest normal
+// number from 16,384 keys on), and dS as 2^e dS, e a power of two from the bound
+// |dP_ij - delta_i| <= 2 |dout_i| max_j |v_j| that puts the bound just below
+// f16's largest number; both factors are taken out of the f32 sums.
+#include "t2h_attn_core.h"
+
+namespace t2h {
+namespace {
+
+constexpr int kPrepRows = 64;     // rows per block of the first pass, and per entry of the maxima
+constexpr float kShiftP = 14.0f;  // f16: P is rounded as 2^kShiftP P
+
+template <typename T> struct HalfRange { static constexpr bool value = false; };
+template <> struct HalfRange<_Float16> { static constexpr bool value = true; };
+
+// Largest of the entries of n rows.
+__device__ __forceinline__ float largest(const float* entries, int64_t n, int lane) {
+    float m = 0.0f;
+    for (int64_t t = lane; t * kPrepRows < n; t += 64) m = fmaxf(m, entries[t]);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    return m;
+}
+// e with 2^e * 2 sqrt(g2 v2) below 2^16, from the largest squared lengths.
+__device__ __forceinline__ float shift_ds(float g2, float v2) {
+    const float b = 2.0f * sqrtf(g2) * sqrtf(v2);
+    int e = 14 - ((int)((__builtin_bit_cast(uint32_t, b) >> 23) & 255u) - 127);
+    e = e > 60 ? 60 : e < -60 ? -60 : e;
+    return (float)e;
+}
+
+// ---- delta and row lengths ----------------------------------------------------
+// A block takes up to kPrepRows rows of one segment and one head of dout and out
+// (or, f16, of v; only keys that count), 16 lanes a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
+    constexpr int E = D / 16;
+    const AttnArgs& f = a.f;
+    const int64_t u = block_linear();
+    if (u >= a.prep_blocks) return;
+    const int m = threadIdx.x & 15, rr = threadIdx.x >> 4;
+    const int64_t qb = a.prep_q_tiles * f.heads;
+    __shared__ float top[16];
+    float most = 0.0f;
+    int32_t b;
+    if (u < qb) {
+        const int head = (int)(u / a.prep_q_tiles);
+        const Rows s = tile_rows<kPrepRows>(f.q_offsets, f.q_rows, f.nbatch, u - head * a.prep_q_tiles, b);
+#pragma unroll
+        for (int i = 0; i < kPrepRows / 16; ++i) {
+            const int64_t row = s.lo + i * 16 + rr;
+            if (row >= s.hi) break;
+            float g[E], o[E];
+            load_elems<T, E>(static_cast<const T*>(a.dout) + row * a.do_row + head * a.do_head + m * E, g);
+            load_elems<T, E>(static_cast<const T*>(f.out) + row * f.o_row + head * f.o_head + m * E, o);
+            float d = 0.0f, g2 = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                d = fmaf(g[e], o[e], d);
+                g2 = fmaf(g[e], g[e], g2);
+            }
+            d = row16_sum(d);
+            if (HalfRange<T>::value) most = fmaxf(most, row16_sum(g2));
+            if (m == 0) {
+                const int64_t at = head * f.q_rows + row;
+                const float lse = f.lse[at];
+                a.delta[at] = d;
+                a.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e - (HalfRange<T>::value ? kShiftP : 0.0f);
+            }
+        }
+    } else {
+        const int64_t w = u - qb;
+        const int head = (int)(w / a.prep_k_tiles);
+        Rows s = tile_rows<kPrepRows>(f.k_offsets, f.k_rows, f.nbatch, w - head * a.prep_k_tiles, b);
+        const int64_t end = segment_keys(f, b).hi;
+        s.hi = end < s.hi ? end : s.hi;
+#pragma unroll
+        for (int i = 0; i < kPrepRows / 16; ++i) {
+            const int64_t row = s.lo + i * 16 + rr;
+            if (row >= s.hi) break;
+            float v[E];
+            load_elems<T, E>(static_cast<const T*>(f.v) + row * f.v_row + head * f.v_head + m * E, v);
+            most = fmaxf(most, row16_sum(sum_sq_all<E>(v)));
+        }
+    }
+    if constexpr (HalfRange<T>::value) {
+        if (m == 0) top[rr] = most;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int i = 1; i < 16; ++i) most = fmaxf(most, top[i]);
+            (u < qb ? a.g_most : a.v_most)[u < qb ? u : u - qb] = most;
+        }
+    }
+}
+
+// ---- dk, dv ---------------------------------------------------------------------
+constexpr int kQT = 64;   // queries per tile
+
+template <typename T, int D, int NW, int NT, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a) {
+    using V8 = typename AttnMma<T>::v8;
+    constexpr int BK = NW * NT * 16;
+    constexpr int kTile = kQT * D * 2;
+    constexpr bool kF16 = HalfRange<T>::value;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile + 4 * kQT * 4];   // q, q, dout, dout, lse2 x 2, delta x 2
+    const AttnArgs& f = a.f;
+    const int64_t p = block_linear();
+    if (p >= a.kv_blocks) return;
+    const int64_t u = xcd_order(p, a.kv_blocks);
+    const int64_t per_head = a.k_tiles * a.kv_split;
+    const int kvh = (int)(u / per_head);
+    const int64_t rem = u - kvh * per_head;
+    const int split = (int)(rem / a.k_tiles);
+    int32_t b;
+    const Rows ks = tile_rows<BK>(f.k_offsets, f.k_rows, f.nbatch, rem - split * a.k_tiles, b);
+    if (ks.lo >= ks.hi) return;
+    const Rows qs = segment_rows(f.q_offsets, f.q_rows, f.nbatch, b);
+    // keys from k_end on do not count: their gradients are zero
+    const Rows seg = segment_keys(f, b);
+    const int64_t k_end = seg.hi;
+
+    const int lane = lane_id(), r = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t k0 = ks.lo + wave * (NT * 16);
+    const bool active = k0 < k_end;
+    const int tiles = (int)((qs.hi - qs.lo + kQT - 1) / kQT);
+    const int total = ks.lo < k_end ? tiles * f.group : 0;
+    const int it0 = SPLIT ? (int)((int64_t)total * split / a.kv_split) : 0;
+    const int it1 = SPLIT ? (int)((int64_t)total * (split + 1) / a.kv_split) : total;
+
+    TileLoad<D, kQT, NW> lq, lg;
+    lq.init(wave, lane, f.q_row);
+    lg.init(wave, lane, a.do_row);
+    const FragAddr<D> fa(lane);
+    const float c = f.scale * kLog2e;
+
+    V8 k[NT][D / 32], v[NT][D / 32];
+    f32x4 dk[D / 16][NT], dv[D / 16][NT];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) dk[i][j] = dv[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float z = 1.0f, shift = 0.0f;
+    if (it0 < it1) {
+        if constexpr (kF16) {
+            float g2 = 0.0f;
+            const int64_t qt0 = first_tile<kPrepRows>(f.q_offsets, f.q_rows, f.nbatch, b);
+            for (int i = 0; i < f.group; ++i)
+                g2 = fmaxf(g2, largest(a.g_most + (kvh * f.group + i) * a.prep_q_tiles + qt0, qs.hi - qs.lo, lane));
+            const int64_t kt0 = first_tile<kPrepRows>(f.k_offsets, f.k_rows, f.nbatch, b);
+            shift = shift_ds(g2, largest(a.v_most + kvh * a.prep_k_tiles + kt0, seg.hi - seg.lo, lane));
+            z = exp2_f(shift - kShiftP);
+        }
+        const auto issue = [&](int it, int st) {
+            const int g = it / tiles;
+            const int head = kvh * f.group + g;
+            const int64_t row = qs.lo + (int64_t)(it - g * tiles) * kQT;
+            lq.issue(static_cast<const uint8_t*>(f.q) + head * f.q_head * 2, row, qs.hi, lds + st * kTile);
+            lg.issue(static_cast<const uint8_t*>(a.dout) + head * a.do_head * 2, row, qs.hi, lds + (2 + st) * kTile);
+            if (wave < 2) {
+                const int64_t at = head * f.q_rows + row, left = qs.hi - row;
+                const float* src = (wave == 0 ? a.lse2 : a.delta) + at;
+                const __amdgpu_buffer_rsrc_t rs = rows_rsrc(reinterpret_cast<const uint8_t*>(src),
+                                                            (uint32_t)(left < kQT ? left : kQT) * 4);
+                rsrc_to_lds4(rs, lds + 4 * kTile + (2 * wave + st) * kQT * 4, (uint32_t)lane * 4);
+            }
+        };
+        issue(it0, 0);
+        if (active) {
+            const uint8_t* kb = static_cast<const uint8_t*>(f.k) + (kvh * f.k_head + k0 * f.k_row) * 2;
+            const uint8_t* vb = static_cast<const uint8_t*>(f.v) + (kvh * f.v_head + k0 * f.v_row) * 2;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                load_own<T, D>(k[j], kb + 16 * j * f.k_row * 2, k_end - k0 - 16 * j, (uint32_t)f.k_row * 2, lane);
+                load_own<T, D>(v[j], vb + 16 * j * f.v_row * 2, k_end - k0 - 16 * j, (uint32_t)f.v_row * 2, lane);
+            }
+        }
+        for (int it = it0; it < it1; ++it) {
+            const int st = (it - it0) & 1;
+            wait_loads<0>();
+            wait_lds_reads();
+            tile_barrier();
+            if (it + 1 < it1) issue(it + 1, 1 - st);
+            if (!active) continue;
+            const uint8_t* qt = lds + st * kTile;
+            const uint8_t* gt = lds + (2 + st) * kTile;
+            const float* ls = reinterpret_cast<const float*>(lds + 4 * kTile) + st * kQT;
+            const float* de = ls + 2 * kQT;
+#pragma unroll
+            for (int s2 = 0; s2 < kQT / 32; ++s2) {
+                f32x4 s[2][NT], d[2][NT];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) s[i][j] = d[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const V8 x = row_frag<T, D>(qt, fa.row, 2 * s2 + i, t);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) s[i][j] = AttnMma<T>::run(x, k[j][t], s[i][j]);
+                    }
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const V8 x = row_frag<T, D>(gt, fa.row, 2 * s2 + i, t);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) d[i][j] = AttnMma<T>::run(x, v[j][t], d[i][j]);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + 32 * s2 + 16 * i + 4 * h);
+                    f32x4 d4 = *reinterpret_cast<const f32x4*>(de + 32 * s2 + 16 * i + 4 * h);
+                    if (kF16) d4 *= z;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[i][j][e] = exp2_f(fmaf(s[i][j][e], c, -l4[e]));
+                            d[i][j][e] = s[i][j][e] * (kF16 ? fmaf(d[i][j][e], z, -d4[e]) : d[i][j][e] - d4[e]);
+                        }
+                }
+                V8 pf[NT], df[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    pf[j] = pack_frag<T>(s[0][j], s[1][j]);
+                    df[j] = pack_frag<T>(d[0][j], d[1][j]);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const V8 x = tr_frag<T, D>(gt, fa.tr, s2, i);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) dv[i][j] = AttnMma<T>::run(x, pf[j], dv[i][j]);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const V8 x = tr_frag<T, D>(qt, fa.tr, s2, i);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) dk[i][j] = AttnMma<T>::run(x, df[j], dk[i][j]);
+                }
+            }
+        }
+    }
+    const float wk = f.scale * (kF16 ? exp2_f(-shift) : 1.0f), wv = kF16 ? exp2_f(-kShiftP) : 1.0f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t row = k0 + 16 * j + r;
+        if (row >= ks.hi) continue;
+        const bool counts = row < k_end;
+        if constexpr (SPLIT) {
+            float* pk = a.part + (((int64_t)split * f.k_rows + row) * a.kv_heads + kvh) * D + 4 * h;
+            float* pv = pk + (int64_t)a.kv_split * f.k_rows * a.kv_heads * D;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                *reinterpret_cast<f32x4*>(pk + 16 * i) = counts ? dk[i][j] * wk : zero;
+                *reinterpret_cast<f32x4*>(pv + 16 * i) = counts ? dv[i][j] * wv : zero;
+            }
+        } else {
+            T* pk = static_cast<T*>(a.dk) + row * a.dk_row + kvh * a.dk_head + 4 * h;
+            T* pv = static_cast<T*>(a.dv) + row * a.dv_row + kvh * a.dv_head + 4 * h;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                typename AttnMma<T>::v4 x, y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = counts ? (T)(dk[i][j][e] * wk) : (T)0.0f;
+                    y[e] = counts ? (T)(dv[i][j][e] * wv) : (T)0.0f;
+                }
+                *reinterpret_cast<typename AttnMma<T>::v4*>(pk + 16 * i) = x;
+                *reinterpret_cast<typename AttnMma<T>::v4*>(pv + 16 * i) = y;
+            }
+        }
+    }
+}
+
+// ---- dq -------------------------------------------------------------------------
+constexpr int kKT = 64;   // keys per tile
+
+template <typename T, int D, int NW, int NT, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, NW / 4) void attn_dq_kernel(AttnBwdArgs a) {
+    using V8 = typename AttnMma<T>::v8;
+    constexpr int BQ = NW * NT * 16;
+    constexpr int kTile = kKT * D * 2;
+    constexpr bool kF16 = HalfRange<T>::value;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];   // k, k, v, v
+    const AttnArgs& f = a.f;
+    const int64_t p = block_linear();
+    if (p >= a.q_blocks) return;
+    const int64_t u = xcd_order(p, a.q_blocks);
+    const int64_t per_head = f.q_tiles * a.q_split;
+    const int head = (int)(u / per_head);
+    const int64_t rem = u - head * per_head;
+    const int split = (int)(rem / f.q_tiles);
+    int32_t b;
+    const Rows qs = tile_rows<BQ>(f.q_offsets, f.q_rows, f.nbatch, rem - split * f.q_tiles, b);
+    if (qs.lo >= qs.hi) return;
+    Rows ks = segment_keys(f, b);
+    const int64_t keys = ks.hi - ks.lo;
+    if constexpr (SPLIT) {
+        const int64_t tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
+        const int64_t t0 = tiles * split / a.q_split, t1 = tiles * (split + 1) / a.q_split;
+        const int64_t hi = ks.lo + t1 * kKT;
+        if (hi < ks.hi) ks.hi = hi;
+        ks.lo += t0 * kKT;
+    }
+    const int n = (int)((ks.hi - ks.lo + kKT - 1) / kKT);
+
+    const int lane = lane_id(), r = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t q0 = qs.lo + wave * (NT * 16);
+    const bool active = q0 < qs.hi;
+    const int kvh = head / f.group;
+    const uint8_t* kb = static_cast<const uint8_t*>(f.k) + kvh * f.k_head * 2;
+    const uint8_t* vb = static_cast<const uint8_t*>(f.v) + kvh * f.v_head * 2;
+    TileLoad<D, kKT, NW> lk, lv;
+    lk.init(wave, lane, f.k_row);
+    lv.init(wave, lane, f.v_row);
+    const FragAddr<D> fa(lane);
+    const float c = f.scale * kLog2e;
+
+    V8 q[NT][D / 32], g[NT][D / 32];
+    f32x4 dq[D / 16][NT];
+    float l2[NT], de[NT], z[NT], w[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) dq[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        l2[j] = INFINITY;
+        de[j] = 0.0f;
+        z[j] = 1.0f;
+        w[j] = f.scale;
+    }
+    if (n > 0) {
+        lk.issue(kb, ks.lo, ks.hi, lds);
+        lv.issue(vb, ks.lo, ks.hi, lds + 2 * kTile);
+        if (active) {
+            float v2 = 0.0f;
+            if constexpr (kF16)
+                v2 = largest(a.v_most + kvh * a.prep_k_tiles + first_tile<kPrepRows>(f.k_offsets, f.k_rows, f.nbatch, b), keys, lane);
+            const uint8_t* qb = static_cast<const uint8_t*>(f.q) + (head * f.q_head + q0 * f.q_row) * 2;
+            const uint8_t* gb = static_cast<const uint8_t*>(a.dout) + (head * a.do_head + q0 * a.do_row) * 2;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                load_own<T, D>(q[j], qb + 16 * j * f.q_row * 2, qs.hi - q0 - 16 * j, (uint32_t)f.q_row * 2, lane);
+                load_own<T, D>(g[j], gb + 16 * j * a.do_row * 2, qs.hi - q0 - 16 * j, (uint32_t)a.do_row * 2, lane);
+                const int64_t row = q0 + 16 * j + r;
+                if (row < qs.hi) {
+                    l2[j] = a.lse2[head * f.q_rows + row];
+                    de[j] = a.delta[head * f.q_rows + row];
+                }
+                if constexpr (kF16) {
+                    float g2 = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) g2 = fmaf((float)g[j][t][e], (float)g[j][t][e], g2);
+                    g2 += __shfl_xor(g2, 16);
+                    g2 += __shfl_xor(g2, 32);
+                    const float e = shift_ds(g2, v2);
+                    z[j] = exp2_f(e - kShiftP);
+                    de[j] *= z[j];
+                    w[j] = f.scale * exp2_f(-e);
+                }
+            }
+        }
+        for (int t = 0; t < n; ++t) {
+            const int st = t & 1;
+            wait_loads<0>();
+            wait_lds_reads();
+            tile_barrier();
+            if (t + 1 < n) {
+                lk.issue(kb, ks.lo + (t + 1) * (int64_t)kKT, ks.hi, lds + (1 - st) * kTile);
+                lv.issue(vb, ks.lo + (t + 1) * (int64_t)kKT, ks.hi, lds + (3 - st) * kTile);
+            }
+            if (!active) continue;
+            const int64_t left = ks.hi - ks.lo - t * (int64_t)kKT;
+            const uint8_t* kt = lds + st * kTile;
+            const uint8_t* vt = lds + (2 + st) * kTile;
+#pragma unroll
+            for (int s2 = 0; s2 < kKT / 32; ++s2) {
+                f32x4 s[2][NT], d[2][NT];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) s[i][j] = d[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const V8 y = row_frag<T, D>(kt, fa.row, 2 * s2 + i, x);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) s[i][j] = AttnMma<T>::run(y, q[j][x], s[i][j]);
+                    }
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const V8 y = row_frag<T, D>(vt, fa.row, 2 * s2 + i, x);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) d[i][j] = AttnMma<T>::run(y, g[j][x], d[i][j]);
+                    }
+                // keys past the last: their score 0 may be far above lse, and P with it beyond any number
+                if (left < kKT) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (32 * s2 + 16 * i + 4 * h + e >= left) {
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) s[i][j][e] = -INFINITY;
+                            }
+                }
+                V8 df[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float pr = exp2_f(fmaf(s[i][j][e], c, -l2[j]));
+                            d[i][j][e] = pr * (kF16 ? fmaf(d[i][j][e], z[j], -de[j]) : d[i][j][e] - de[j]);
+                        }
+                    df[j] = pack_frag<T>(d[0][j], d[1][j]);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const V8 x = tr_frag<T, D>(kt, fa.tr, s2, i);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) dq[i][j] = AttnMma<T>::run(x, df[j], dq[i][j]);
+                }
+            }
+        }
+    }
+    if (!active) return;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t row = q0 + 16 * j + r;
+        if (row >= qs.hi) continue;
+        if constexpr (SPLIT) {
+            float* po = a.part + (((int64_t)split * f.q_rows + row) * f.heads + head) * D + 4 * h;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(po + 16 * i) = dq[i][j] * w[j];
+        } else {
+            T* po = static_cast<T*>(a.dq) + row * a.dq_row + head * a.dq_head + 4 * h;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                typename AttnMma<T>::v4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (T)(dq[i][j][e] * w[j]);
+                *reinterpret_cast<typename AttnMma<T>::v4*>(po + 16 * i) = x;
+            }
+        }
+    }
+}
+
+// Sum of the parts [nsplit, rows, heads, D] in order; blockIdx.z: part set
+// (dk, dv) and output.
+struct SumArgs {
+    const float* part[2];
+    void* out[2];
+    int64_t row_stride[2], head_stride[2];
+    const int64_t* offsets;   // rows outside the segments are left alone
+    int64_t rows;
+    int32_t heads, nsplit, nbatch;
+};
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_sum_kernel(SumArgs a) {
+    constexpr int E = D / 16;
+    const int64_t u = block_linear() * 16 + threadIdx.x / 16;
+    if (u >= a.rows * a.heads) return;
+    const int64_t row = u / a.heads;
+    const int head = (int)(u - row * a.heads);
+    if (a.offsets != nullptr && (row < a.offsets[0] || row >= a.offsets[a.nbatch])) return;
+    const int m = threadIdx.x & 15, w = blockIdx.z;
+    float acc[E] = {};
+    for (int s = 0; s < a.nsplit; ++s) {
+        float v[E];
+        load_params<E>(a.part[w] + (((int64_t)s * a.rows + row) * a.heads + head) * D + m * E, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += v[e];
+    }
+    store_elems<T, E>(static_cast<T*>(a.out[w]) + row * a.row_stride[w] + head * a.head_stride[w] + m * E, acc);
+}
+
+constexpr int kDqWaves = 8, kDqTiles = 2;
+#ifndef T2H_DKV_WAVES
+#define T2H_DKV_WAVES 4
+#define T2H_DKV_TILES 2
+#endif
+constexpr int kDkvWaves = T2H_DKV_WAVES, kDkvTiles = T2H_DKV_TILES;
+constexpr int kBQ = kDqWaves * kDqTiles * 16, kBK = kDkvWaves * kDkvTiles * 16;
+
+template <typename T, int D>
+hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
+    AttnArgs& f = a.f;
+    if (a.prep_blocks > 0) hipLaunchKernelGGL((attn_prep_kernel<T, D>), grid_1d(a.prep_blocks), dim3(256), 0, s, a);
+    a.k_tiles = tile_count(f.k_offsets, f.k_rows, f.nbatch, kBK);
+    a.kv_blocks = a.k_tiles * a.kv_split * a.kv_heads;
+    if (a.kv_blocks > 0) {
+        if (a.kv_split > 1) {
+            hipLaunchKernelGGL((attn_dkv_kernel<T, D, kDkvWaves, kDkvTiles, true>), grid_1d(a.kv_blocks), dim3(kDkvWaves * 64), 0, s, a);
+            SumArgs m{};
+            m.part[0] = a.part;
+            m.part[1] = a.part + a.kv_split * f.k_rows * a.kv_heads * D;
+            m.out[0] = a.dk;
+            m.out[1] = a.dv;
+            m.row_stride[0] = a.dk_row;
+            m.row_stride[1] = a.dv_row;
+            m.head_stride[0] = a.dk_head;
+            m.head_stride[1] = a.dv_head;
+            m.offsets = f.k_offsets;
+            m.rows = f.k_rows;
+            m.heads = a.kv_heads;
+            m.nsplit = a.kv_split;
+            m.nbatch = f.nbatch;
+            dim3 grid = grid_1d((m.rows * m.heads + 15) / 16);
+            grid.z = 2;
+            hipLaunchKernelGGL((attn_sum_kernel<T, D>), grid, dim3(256), 0, s, m);
+        } else {
+            hipLaunchKernelGGL((attn_dkv_kernel<T, D, kDkvWaves, kDkvTiles, false>), grid_1d(a.kv_blocks), dim3(kDkvWaves * 64), 0, s, a);
+        }
+    }
+    f.q_tiles = tile_count(f.q_offsets, f.q_rows, f.nbatch, kBQ);
+    a.q_blocks = f.q_tiles * a.q_split * f.heads;
+    if (a.q_blocks > 0) {
+        if (a.q_split > 1) {
+            hipLaunchKernelGGL((attn_dq_kernel<T, D, kDqWaves, kDqTiles, true>), grid_1d(a.q_blocks), dim3(kDqWaves * 64), 0, s, a);
+            SumArgs m{};
+            m.part[0] = a.part;
+            m.out[0] = a.dq;
+            m.row_stride[0] = a.dq_row;
+            m.head_stride[0] = a.dq_head;
+            m.offsets = f.q_offsets;
+            m.rows = f.q_rows;
+            m.heads = f.heads;
+            m.nsplit = a.q_split;
+            m.nbatch = f.nbatch;
+            hipLaunchKernelGGL((attn_sum_kernel<T, D>), grid_1d((m.rows * m.heads + 15) / 16), dim3(256), 0, s, m);
+        } else {
+            hipLaunchKernelGGL((attn_dq_kernel<T, D, kDqWaves, kDqTiles, false>), grid_1d(a.q_blocks), dim3(kDqWaves * 64), 0, s, a);
+        }
+    }
+    return hipGetLastError();
+}
+
+int splits(int64_t tiles, int64_t stream, int per) {
+    int64_t n = device_cu_count() / (tiles > 0 ? tiles : 1);
+    if (n > stream / per) n = stream / per;
+    if (n > 64) n = 64;
+    return n < 1 ? 1 : (int)n;
+}
+int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+// The workspace: delta and lse2 [heads, q_rows], the maxima (f16), then the
+// parts of whichever of dk, dv and dq are split (one after the other).
+int64_t attn_bwd_plan(AttnBwdArgs& a, void* workspace) {
+    AttnArgs& f = a.f;
+    a.prep_q_tiles = tile_count(f.q_offsets, f.q_rows, f.nbatch, kPrepRows);
+    a.prep_k_tiles = tile_count(f.k_offsets, f.k_rows, f.nbatch, kPrepRows);
+    a.prep_blocks = a.prep_q_tiles * f.heads + (f.dtype == T2H_F16 ? a.prep_k_tiles * a.kv_heads : 0);
+    const int64_t kt = (f.k_rows / f.nbatch + kBK - 1) / kBK * f.nbatch, qt = (f.q_rows / f.nbatch + kBQ - 1) / kBQ * f.nbatch;
+    a.kv_split = splits(kt * a.kv_heads, f.q_rows / f.nbatch * f.group, 2 * kQT);
+    a.q_split = splits(qt * f.heads, f.k_rows / f.nbatch, 2 * kKT);
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    int64_t at = 0;
+    const auto take = [&](int64_t floats) {
+        float* p = reinterpret_cast<float*>(w + at);
+        at += up256(floats * 4);
+        return p;
+    };
+    a.delta = take(f.q_rows * f.heads);
+    a.lse2 = take(f.q_rows * f.heads);
+    a.g_most = take((f.q_rows / kPrepRows + f.nbatch) * f.heads);     // as many with offsets as without
+    a.v_most = take((f.k_rows / kPrepRows + f.nbatch) * a.kv_heads);
+    const int64_t pk = a.kv_split > 1 ? 2 * a.kv_split * f.k_rows * a.kv_heads * f.head_dim : 0;
+    const int64_t pq = a.q_split > 1 ? a.q_split * f.q_rows * f.heads * f.head_dim : 0;
+    a.part = take(pk > pq ? pk : pq);
+    return at;
+}
+
+hipError_t launch_attn_bwd(const AttnBwdArgs& a, hipStream_t s) {
+    if (a.f.dtype == T2H_F16) return a.f.head_dim == 128 ? launch_d<_Float16, 128>(a, s) : launch_d<_Float16, 64>(a, s);
+    return a.f.head_dim == 128 ? launch_d<__bf16, 128>(a, s) : launch_d<__bf16, 64>(a, s);
+}
+
+}  // namespace t2h

@@ -61,7 +61,8 @@ template <typename... A> PyObject* invoke(int32_t (*f)(A...), PyObject* const* a
     X(t2h_attn_pack) X(t2h_rope_phases) X(t2h_activation) X(t2h_qkv_linear_pack) X(t2h_linear_gate_residual)           \
     X(t2h_linear) X(t2h_gate_residual) X(t2h_gate_residual_ln_modulate) X(t2h_timestep_embedding)                      \
     X(t2h_coords_to_offsets) X(t2h_modulation_add) X(t2h_flow_euler_step) X(t2h_ln_mod_rows)                           \
-    X(t2h_gate_add_bias_rows) X(t2h_block_join_ln)
+    X(t2h_gate_add_bias_rows) X(t2h_block_join_ln) X(t2h_attention) X(t2h_attention_backward)                          \
+    X(t2h_qk_rmsnorm_rope_backward)
 
 #define T2H_WRAP(name)                                                                                                 \
     decltype(&name) p_##name = nullptr;                                                                                \

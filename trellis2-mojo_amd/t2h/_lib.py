@@ -40,6 +40,13 @@ _SIGNATURES = {
                                   c_i64, c_p, c_i32, c_i32, c_p],
     "t2h_attn_pack": [c_p, c_p, c_p, c_i64, c_i64, c_i32, c_i32, c_i32, c_p, c_p, c_p, c_p, c_p, c_i32, c_p, c_i32,
                       c_i32, c_p, c_i64, c_p, c_i32, c_i32, c_p, c_i64, c_p, c_p, c_i64, c_i32, c_p],
+    "t2h_attention": [c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_f32, c_p, c_p, c_p,
+                      c_i32, c_p, c_i64, c_p],
+    "t2h_attention_backward": [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i32, c_i32, c_i32,
+                               c_i32, c_f32, c_p, c_p, c_p, c_i32, c_p, c_i64, c_p],
+    "t2h_qk_rmsnorm_rope_backward": [c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32,
+                                     c_p, c_p, c_p, c_p, c_i32, c_p, c_i32, c_i32, c_p, c_i64, c_p, c_i32, c_i32, c_p,
+                                     c_p, c_p, c_p, c_p, c_i64, c_p],
     "t2h_rope_freqs": [c_i32, c_i32, c_f64, c_f64, c_p, c_i32],
     "t2h_rope_phases": [c_p, c_i64, c_i32, c_p, c_i32, c_i32, c_p, c_p, c_i32, c_i32, c_p],
     "t2h_activation": [c_p, c_p, c_p, c_i64, c_i32, c_i32, c_i32, c_p],
@@ -69,7 +76,14 @@ _SIGNATURES = {
     "t2h_h_timestep_embedding": [c_p, c_p, c_i64, c_i32, c_f64],
     "t2h_h_coords_to_offsets": [c_p, c_i64, c_i32, c_i32, c_p],
 }
-EXPORTED = ["t2h_version", "t2h_last_error", "t2h_flow_euler_workspace", *_SIGNATURES]
+# byte counts (int64) instead of a status
+_SIZES = {
+    "t2h_flow_euler_workspace": [c_i64, c_i64, c_i32],
+    "t2h_attention_workspace": [c_i64, c_i64, c_i32, c_i32, c_i32, c_i32],
+    "t2h_attention_backward_workspace": [c_i64, c_i64, c_i32, c_i32, c_i32, c_i32],
+    "t2h_qk_rmsnorm_rope_backward_workspace": [c_i64, c_i32, c_i32, c_i32],
+}
+EXPORTED = ["t2h_version", "t2h_last_error", *_SIZES, *_SIGNATURES]
 
 _lib = None
 _calls = {}     # name -> callable returning the status, filled by load()
@@ -95,8 +109,10 @@ def load(path: str | None = None):
     L.t2h_version.argtypes = []
     L.t2h_last_error.restype = ctypes.c_char_p
     L.t2h_last_error.argtypes = []
-    L.t2h_flow_euler_workspace.restype = c_i64
-    L.t2h_flow_euler_workspace.argtypes = [c_i64, c_i64, c_i32]
+    for name, args in _SIZES.items():
+        fn = getattr(L, name)
+        fn.restype = c_i64
+        fn.argtypes = args
     for name, args in _SIGNATURES.items():
         fn = getattr(L, name)
         fn.restype = c_i32

@@ -7,6 +7,8 @@ CPU tensor raises.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 from typing import Optional, Sequence
 
@@ -315,6 +317,196 @@ def attn_pack(q=None, k=None, v=None, mp: int = 0, lp: int = 0, bias_q=None, bia
          p(qh), mp, p(ko), p(vh), lp, int(bool(k_transposed)), _stream())
     del hold
     return qh, ko, vh
+
+
+# ---- attention -------------------------------------------------------------------
+def _same_device(ref: torch.Tensor, tensors, what: str) -> None:
+    """Every tensor on ref's device, and that the current one (the launch's)."""
+    _dev(ref, what)
+    if ref.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors must be on the current device")
+    for t in tensors:
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{what}: tensors are on different devices")
+
+
+def _attn_operand(t: torch.Tensor, rows: int, h: int, d: int, dtype, what: str, name: str):
+    """[rows, H, D] with unit stride on D -> (row stride, head stride) in elements."""
+    if t.dim() != 3 or t.shape != (rows, h, d) or t.dtype != dtype:
+        raise ValueError(f"{what}: {name} must be [{rows}, {h}, {d}] of {dtype}")
+    if t.stride(2) != 1 and t.numel() > 0:
+        raise ValueError(f"{what}: {name} must have unit stride on its last dim")
+    # a dimension of one has no stride of its own
+    return (t.stride(0) if rows > 1 else 0, t.stride(1) if h > 1 else 0)
+
+
+def _attn_segments(what: str, nbatch: int, **offsets):
+    for name, t in offsets.items():
+        n = nbatch if name == "k_lens" else nbatch + 1
+        if t is not None and (t.dtype != torch.int64 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous int64 [{n}]")
+
+
+def _attn_shapes(q, k, what: str):
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"{what}: expected q [rows, H, D] and k, v [rows, Hkv, D]")
+    return *q.shape, k.shape[0], k.shape[1]
+
+
+def _strides_host(pairs):
+    a = (ctypes.c_int64 * (2 * len(pairs)))(*(s for p in pairs for s in p))
+    return a, ctypes.addressof(a)
+
+
+def _attn_workspace(ws, need: int, device, what: str):
+    if ws is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if ws.dtype != torch.uint8 or not ws.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous uint8")
+    return ws
+
+
+@functools.lru_cache(maxsize=256)
+def attention_workspace(q_rows: int, k_rows: int, heads: int, kv_heads: int, head_dim: int, nbatch: int = 1) -> int:
+    """Bytes of workspace with which attention() may split its keys (0: no use for any)."""
+    n = int(_lib.load().t2h_attention_workspace(q_rows, k_rows, heads, kv_heads, head_dim, nbatch))
+    if n < 0:
+        raise ValueError(_lib.load().t2h_last_error().decode(errors="replace"))
+    return n
+
+
+@functools.lru_cache(maxsize=256)
+def attention_backward_workspace(q_rows: int, k_rows: int, heads: int, kv_heads: int, head_dim: int,
+                                 nbatch: int = 1) -> int:
+    """Bytes of workspace that attention_backward() needs."""
+    n = int(_lib.load().t2h_attention_backward_workspace(q_rows, k_rows, heads, kv_heads, head_dim, nbatch))
+    if n < 0:
+        raise ValueError(_lib.load().t2h_last_error().decode(errors="replace"))
+    return n
+
+
+def attention(q, k, v, scale: Optional[float] = None, q_offsets=None, k_offsets=None, k_lens=None, nbatch: int = 1,
+              need_lse: bool = False, out=None, workspace=None):
+    """softmax(scale * q k^T) v within segments: q [rows, H, D], k, v [rows,
+    Hkv, D] float16/bfloat16 (H a multiple of Hkv, D 64 or 128; views of a
+    packed qkv, or a head-major tensor transposed to [rows, H, D], are read in
+    place), scale None = 1/sqrt(D). Segments: q_offsets / k_offsets int64
+    [nbatch + 1] on the device, or nbatch equal shares of a side without them;
+    k_lens int64 [nbatch]: only the first k_lens[b] keys of a segment count.
+    Returns out [rows, H, D], with need_lse (out, lse [H, rows] float32). A row
+    without keys gets 0 (lse -inf); rows outside the segments are not written.
+    workspace: attention_workspace() bytes (uint8), else allocated here."""
+    what = "attention"
+    _same_device(q, (k, v, q_offsets, k_offsets, k_lens, out, workspace), what)
+    dt = _dtype(q, what)
+    rows, h, d, krows, kvh = _attn_shapes(q, k, what)
+    _attn_segments(what, nbatch, q_offsets=q_offsets, k_offsets=k_offsets, k_lens=k_lens)
+    if out is None:
+        out = torch.empty((rows, h, d), dtype=q.dtype, device=q.device)
+    hold, sp = _strides_host((_attn_operand(q, rows, h, d, q.dtype, what, "q"),
+                              _attn_operand(k, krows, kvh, d, q.dtype, what, "k"),
+                              _attn_operand(v, krows, kvh, d, q.dtype, what, "v"),
+                              _attn_operand(out, rows, h, d, q.dtype, what, "out")))
+    lse = torch.empty((h, rows), dtype=torch.float32, device=q.device) if need_lse else None
+    ws = _attn_workspace(workspace, attention_workspace(rows, krows, h, kvh, d, nbatch), q.device, what)
+    call("t2h_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), sp, rows, krows, h, kvh,
+         d, dt, d ** -0.5 if scale is None else float(scale), _ptr(q_offsets), _ptr(k_offsets), _ptr(k_lens),
+         int(nbatch), _ptr(ws), ws.numel() if ws is not None else 0, _stream())
+    del hold
+    return (out, lse) if need_lse else out
+
+
+def attention_backward(dout, q, k, v, out, lse, scale: Optional[float] = None, q_offsets=None, k_offsets=None,
+                       k_lens=None, nbatch: int = 1, dq=None, dk=None, dv=None, workspace=None):
+    """(dq, dk, dv) of attention() from the gradient of its output, its
+    operands, its out and its lse; scale and segments as given there. dq, dk,
+    dv may be given as views of a packed buffer. Keys that do not count get
+    zeros; rows outside the segments are not written. workspace:
+    attention_backward_workspace() bytes (uint8), else allocated here."""
+    what = "attention_backward"
+    _same_device(q, (dout, k, v, out, lse, q_offsets, k_offsets, k_lens, dq, dk, dv, workspace), what)
+    dt = _dtype(q, what)
+    rows, h, d, krows, kvh = _attn_shapes(q, k, what)
+    _attn_segments(what, nbatch, q_offsets=q_offsets, k_offsets=k_offsets, k_lens=k_lens)
+    if lse.dtype != torch.float32 or lse.shape != (h, rows) or not lse.is_contiguous():
+        raise ValueError(f"{what}: lse must be contiguous float32 [{h}, {rows}]")
+    mk = lambda r, n: torch.empty((r, n, d), dtype=q.dtype, device=q.device)
+    dq = mk(rows, h) if dq is None else dq
+    dk = mk(krows, kvh) if dk is None else dk
+    dv = mk(krows, kvh) if dv is None else dv
+    qside = lambda t, name: _attn_operand(t, rows, h, d, q.dtype, what, name)
+    kside = lambda t, name: _attn_operand(t, krows, kvh, d, q.dtype, what, name)
+    hold, sp = _strides_host((qside(q, "q"), kside(k, "k"), kside(v, "v"), qside(out, "out"), qside(dout, "dout"),
+                              qside(dq, "dq"), kside(dk, "dk"), kside(dv, "dv")))
+    ws = _attn_workspace(workspace, attention_backward_workspace(rows, krows, h, kvh, d, nbatch), q.device, what)
+    call("t2h_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+         dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), sp, rows, krows, h, kvh, d, dt,
+         d ** -0.5 if scale is None else float(scale), _ptr(q_offsets), _ptr(k_offsets), _ptr(k_lens), int(nbatch),
+         _ptr(ws), ws.numel() if ws is not None else 0, _stream())
+    del hold
+    return dq, dk, dv
+
+
+def qk_rmsnorm_rope_backward(dq=None, dk=None, q=None, k=None, gamma_q=None, gamma_k=None, bias_q=None, bias_k=None,
+                             freqs=None, pos_dim: int = 3, phases=None, coords=None, grid_res: int = 0,
+                             use_rope: bool = True, in_place: bool = False, workspace=None):
+    """Gradients of qk_rmsnorm_rope() from those of its outputs, dq / dk
+    [rows, H, D] (views allowed; either may be None), and its inputs q / k
+    (needed where a gamma is given). Returns (dq_in, dk_in, dgamma_q, dgamma_k,
+    dbias_q, dbias_k), None where the forward had no such argument; dgamma and
+    dbias float32 [H, D]. in_place: dq_in / dk_in overwrite dq / dk."""
+    what = "qk_rmsnorm_rope_backward"
+    ref = dq if dq is not None else dk
+    if ref is None:
+        raise ValueError(f"{what}: dq and dk are both None")
+    _same_device(ref, (dq, dk, q, k, gamma_q, gamma_k, bias_q, bias_k, phases, coords, workspace), what)
+    rows, h, d, dy_stride = _heads_view(ref, what)
+    dt = _dtype(ref, what)
+    if dk is not None and dk is not ref and (_heads_view(dk, what) != (rows, h, d, dy_stride) or dk.dtype != ref.dtype):
+        raise ValueError(f"{what}: dq/dk layouts differ")
+    in_stride = 0
+    for g, x, gm in ((dq, q, gamma_q), (dk, k, gamma_k)):
+        if g is None:
+            continue
+        if x is None:
+            if gm is not None:
+                raise ValueError(f"{what}: the norm's gradient needs its input")
+            continue
+        r2, h2, d2, s2 = _heads_view(x, what)
+        if (r2, h2, d2) != (rows, h, d) or x.dtype != ref.dtype or in_stride not in (0, s2):
+            raise ValueError(f"{what}: q/k layouts differ")
+        in_stride = s2
+    for t in (gamma_q, gamma_k, bias_q, bias_k):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != h * d or not t.is_contiguous()):
+            raise ValueError(f"{what}: gamma/bias must be contiguous float32 [H, D]")
+    mk = lambda t: None if t is None else t if in_place else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    dqi, dki = mk(dq), mk(dk)
+    din_stride = dy_stride if in_place else h * d
+    par = lambda t, g: torch.empty((h, d), dtype=torch.float32, device=ref.device) if t is not None and g is not None else None
+    dgq, dgk, dbq, dbk = par(gamma_q, dq), par(gamma_k, dk), par(bias_q, dq), par(bias_k, dk)
+    hold, fp, fd = _host_freqs(freqs if freqs is not None else [])
+    ph_rows = 0
+    if phases is not None:
+        if phases.dtype != torch.float32 or not phases.is_contiguous() or phases.shape[-2:] != (d // 2, 2):
+            raise ValueError("apply_rotary_embedding: phases shape mismatch")
+        ph_rows = phases.numel() // d
+    cc = 0
+    if coords is not None:
+        if coords.dtype != torch.int32 or not coords.is_contiguous() or coords.shape[0] != rows:
+            raise ValueError(f"{what}: coords must be contiguous int32 [rows, 1+pos_dim]")
+        cc = coords.shape[1]
+    ws = workspace
+    if any(t is not None for t in (dgq, dgk, dbq, dbk)):
+        n = (dq is not None) + (dk is not None)
+        need = int(_lib.load().t2h_qk_rmsnorm_rope_backward_workspace(rows, h, d, n))
+        ws = _attn_workspace(ws, max(need, 16), ref.device, what)
+    p = _ptr
+    call("t2h_qk_rmsnorm_rope_backward", p(q) if dq is not None else None, p(k) if dk is not None else None, p(dq), p(dk),
+         p(dqi), p(dki), rows, in_stride, dy_stride, din_stride, h, d, dt, p(bias_q), p(bias_k), p(gamma_q), p(gamma_k),
+         int(bool(use_rope)), fp, fd, int(pos_dim), p(phases), ph_rows, p(coords), cc, int(grid_res), p(dgq), p(dgk),
+         p(dbq), p(dbk), p(ws), ws.numel() if ws is not None else 0, _stream())
+    del hold
+    return dqi, dki, dgq, dgk, dbq, dbk
 
 
 def qkv_linear_pack(x, weight, heads: int, bias=None, gamma_q=None, gamma_k=None, mp: int = 0, lp: int = 0,
