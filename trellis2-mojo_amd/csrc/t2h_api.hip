@@ -521,11 +521,18 @@ int32_t attn_sizes(const char* fn, int64_t q_rows, int64_t k_rows, int32_t heads
     if (heads % kv_heads != 0) return fail(T2H_EINVAL, "%s: heads must be a multiple of kv_heads", fn);
     if (head_dim != 64 && head_dim != 128) return fail(T2H_EUNSUPPORTED, "%s: head_dim must be 64 or 128", fn);
     if (nbatch < 1) return fail(T2H_EINVAL, "%s: nbatch < 1", fn);
-    if (q_rows > INT32_MAX || k_rows > INT32_MAX) return fail(T2H_EUNSUPPORTED, "%s: more than 2^31 - 1 rows", fn);
+    if (q_rows > INT32_MAX - 65536 || k_rows > INT32_MAX - 65536)
+        return fail(T2H_EUNSUPPORTED, "%s: more than 2^31 - 65537 rows", fn);
     // block numbers are 32-bit, with up to 64 parts of each tile
     if ((q_rows / 64 + nbatch) * heads >= INT32_MAX / 64 || (k_rows / 64 + nbatch) * kv_heads >= INT32_MAX / 64)
         return fail(T2H_EUNSUPPORTED, "%s: too many tiles", fn);
     return T2H_OK;
+}
+
+void attn_sides(AttnArgs& a, const int64_t* q_offsets, const int64_t* k_offsets, int32_t nbatch) {
+    a.qs = {q_offsets, (int32_t)a.q_rows, (int32_t)(a.q_rows / nbatch)};
+    a.ks = {k_offsets, (int32_t)a.k_rows, (int32_t)(a.k_rows / nbatch)};
+    a.nbatch = nbatch;
 }
 
 // One tensor's strides (0 = contiguous [rows, heads, head_dim]) and alignment.
@@ -568,10 +575,8 @@ int32_t attn_common(const char* fn, AttnArgs& a, const void* q, const void* k, c
     a.head_dim = head_dim;
     a.dtype = dtype;
     a.scale = scale;
-    a.q_offsets = q_offsets;
-    a.k_offsets = k_offsets;
+    attn_sides(a, q_offsets, k_offsets, nbatch);
     a.k_lens = k_lens;
-    a.nbatch = nbatch;
     return T2H_OK;
 }
 
@@ -589,7 +594,7 @@ int64_t t2h_attention_workspace(int64_t q_rows, int64_t k_rows, int32_t heads, i
     a.heads = heads;
     a.group = heads / kv_heads;
     a.head_dim = head_dim;
-    a.nbatch = nbatch;
+    attn_sides(a, nullptr, nullptr, nbatch);
     return attn_split_bytes(a, attn_splits(a));
 }
 
@@ -626,7 +631,7 @@ int64_t t2h_attention_backward_workspace(int64_t q_rows, int64_t k_rows, int32_t
     a.f.heads = heads;
     a.f.group = heads / kv_heads;
     a.f.head_dim = head_dim;
-    a.f.nbatch = nbatch;
+    attn_sides(a.f, nullptr, nullptr, nbatch);
     a.kv_heads = kv_heads;
     return attn_bwd_plan(a, nullptr);
 }

@@ -8,8 +8,12 @@
 namespace t2h {
 
 // Attention and its backward pass (t2h_attention, t2h_attention_backward).
-// Strides in elements; row b of a side's segments from its offsets, or nbatch
-// equal shares.
+// Strides in elements. A side's segments: from its offsets, or nbatch equal shares.
+struct AttnSide {
+    const int64_t* offsets;  // [nbatch + 1] or nullptr
+    int32_t rows;
+    int32_t share;           // rows / nbatch
+};
 struct AttnArgs {
     const void* q;           // [q_rows, heads, head_dim]
     const void* k;           // [k_rows, kv_heads, head_dim]
@@ -23,15 +27,14 @@ struct AttnArgs {
     int32_t head_dim;
     int32_t dtype;
     float scale;
-    const int64_t* q_offsets;
-    const int64_t* k_offsets;
+    AttnSide qs, ks;
     const int64_t* k_lens;   // [nbatch] keys of a segment that count, or nullptr
     int32_t nbatch;
     int32_t nsplit;          // parts of a segment's keys, joined afterwards
     float* part;             // workspace: [nsplit, q_rows, heads, head_dim] parts' outputs
     float* part_lse;         // workspace: [nsplit, heads, q_rows], log2
-    int64_t q_tiles;         // set by the launcher: numbers of query tiles
-    int64_t nblocks;         // set by the launcher
+    int32_t q_tiles;         // set by the launcher: numbers of query tiles
+    int32_t nblocks;         // set by the launcher
 };
 
 struct AttnBwdArgs {
@@ -49,8 +52,8 @@ struct AttnBwdArgs {
     float* g_most;           // [heads, prep_q_tiles] f16: largest squared row length of dout in each tile
     float* v_most;           // [kv_heads, prep_k_tiles]   ... of v
     float* part;
-    int64_t prep_q_tiles, prep_k_tiles, prep_blocks;
-    int64_t k_tiles, kv_blocks, q_blocks;   // set by the launcher
+    int32_t prep_q_tiles, prep_k_tiles, prep_blocks;
+    int32_t k_tiles, kv_blocks, q_blocks;   // set by the launcher
 };
 
 // Backward pass of the q/k epilogue (t2h_qk_rmsnorm_rope_backward).

@@ -20,27 +20,26 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];   // K, K, V, V
     const int64_t p = block_linear();
     if (p >= a.nblocks) return;
-    const int64_t u = xcd_order(p, a.nblocks);
-    const int64_t per_head = a.q_tiles * a.nsplit;
-    const int head = (int)(u / per_head);
-    const int64_t rem = u - head * per_head;
-    const int split = (int)(rem / a.q_tiles);
-    int32_t b;
-    const Rows qs = tile_rows<BQ>(a.q_offsets, a.q_rows, a.nbatch, rem - split * a.q_tiles, b);
+    const int u = xcd_order((int)p, a.nblocks);
+    const int per_head = a.q_tiles * a.nsplit;
+    const int head = u / per_head;
+    const int rem = u - head * per_head;
+    const int split = SPLIT ? rem / a.q_tiles : 0;
+    int b;
+    const Rows qs = tile_rows<BQ>(a.qs, a.nbatch, rem - split * a.q_tiles, b);
     if (qs.lo >= qs.hi) return;
     Rows ks = segment_keys(a, b);
     if constexpr (SPLIT) {
-        const int64_t tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
-        const int64_t t0 = tiles * split / a.nsplit, t1 = tiles * (split + 1) / a.nsplit;
-        const int64_t hi = ks.lo + t1 * kKT;
-        if (hi < ks.hi) ks.hi = hi;
+        const int tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
+        const int t0 = (int)((int64_t)tiles * split / a.nsplit), t1 = (int)((int64_t)tiles * (split + 1) / a.nsplit);
+        if (t1 < tiles) ks.hi = ks.lo + t1 * kKT;
         ks.lo += t0 * kKT;
     }
-    const int n = (int)((ks.hi - ks.lo + kKT - 1) / kKT);
+    const int n = ks.hi > ks.lo ? (ks.hi - ks.lo + kKT - 1) / kKT : 0;
 
     const int lane = lane_id(), r = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t q0 = qs.lo + wave * 32;
+    const int q0 = qs.lo + wave * 32;
     const bool active = q0 < qs.hi;
     const int kvh = head / a.group;
     const uint8_t* kb = static_cast<const uint8_t*>(a.k) + kvh * a.k_head * 2;
@@ -63,7 +62,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
         if (active) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                load_own<T, D>(q[j], static_cast<const uint8_t*>(a.q) + head * a.q_head * 2 + (q0 + 16 * j) * a.q_row * 2,
+                load_own<T, D>(q[j], static_cast<const uint8_t*>(a.q) + head * a.q_head * 2 + (int64_t)(q0 + 16 * j) * a.q_row * 2,
                                qs.hi - q0 - 16 * j, (uint32_t)a.q_row * 2, lane);
         }
         wait_loads<0>();
@@ -122,7 +121,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
         };
         if (active) {
             scores(lds, s);
-            if (n == 1) mask(s, (int)(ks.hi - ks.lo));
+            if (n == 1) mask(s, ks.hi - ks.lo);
             follow(s);
         }
         for (int t = 0; t < n; ++t) {
@@ -130,8 +129,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
             wait_lds_reads();
             tile_barrier();
             const int st = t & 1;
-            if (t + 1 < n) lv.issue(vb, ks.lo + (t + 1) * (int64_t)kKT, ks.hi, lds + (3 - st) * kTile);
-            if (t + 2 < n) lk.issue(kb, ks.lo + (t + 2) * (int64_t)kKT, ks.hi, lds + st * kTile);
+            if (t + 1 < n) lv.issue(vb, ks.lo + (t + 1) * kKT, ks.hi, lds + (3 - st) * kTile);
+            if (t + 2 < n) lk.issue(kb, ks.lo + (t + 2) * kKT, ks.hi, lds + st * kTile);
             if (!active) continue;
             f32x4 sn[4][2];
             if (t + 1 < n) scores(lds + (1 - st) * kTile, sn);
@@ -161,7 +160,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
             if (t + 1 < n) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[i][0] = sn[i][0], s[i][1] = sn[i][1];
-                if (t + 2 == n) mask(s, (int)(ks.hi - ks.lo - (t + 1) * (int64_t)kKT));
+                if (t + 2 == n) mask(s, ks.hi - ks.lo - (t + 1) * kKT);
                 follow(s);
             }
         }
@@ -171,7 +170,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
     for (int j = 0; j < 2; ++j) {
         l[j] += __shfl_xor(l[j], 16);
         l[j] += __shfl_xor(l[j], 32);
-        const int64_t row = q0 + 16 * j + r;
+        const int row = q0 + 16 * j + r;
         if (row >= qs.hi) continue;
         const float inv = l[j] == 0.0f ? 0.0f : 1.0f / l[j];
         const float lse2 = l[j] == 0.0f ? -INFINITY : mc[j] + __builtin_amdgcn_logf(l[j]);
@@ -182,7 +181,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
             for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(po + 16 * i) = o[i][j] * inv;
         } else {
             if (a.lse != nullptr && h == 0) a.lse[head * a.q_rows + row] = lse2 * kLn2;
-            T* po = static_cast<T*>(a.out) + row * a.o_row + head * a.o_head + 4 * h;
+            T* po = static_cast<T*>(a.out) + (int64_t)row * a.o_row + head * a.o_head + 4 * h;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 typename AttnMma<T>::v4 w;
@@ -204,7 +203,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int64_t row = u / a.heads;
     const int head = (int)(u - row * a.heads);
     const int m = threadIdx.x & 15;
-    if (a.q_offsets != nullptr && (row < a.q_offsets[0] || row >= a.q_offsets[a.nbatch])) return;
+    if (a.qs.offsets != nullptr && (row < a.qs.offsets[0] || row >= a.qs.offsets[a.nbatch])) return;
     float top = -INFINITY;
     for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.part_lse[((int64_t)s * a.heads + head) * a.q_rows + row]);
     float acc[E] = {}, sum = 0.0f;
@@ -220,7 +219,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= inv;
-    store_elems<T, E>(static_cast<T*>(a.out) + row * a.o_row + head * a.o_head + m * E, acc);
+    store_elems<T, E>(static_cast<T*>(a.out) + (int64_t)row * a.o_row + head * a.o_head + m * E, acc);
     if (a.lse != nullptr && m == 0)
         a.lse[head * a.q_rows + row] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
@@ -229,7 +228,7 @@ constexpr int kWaves = 8;
 
 template <typename T, int D>
 hipError_t launch_d(AttnArgs a, hipStream_t s) {
-    a.q_tiles = tile_count(a.q_offsets, a.q_rows, a.nbatch, kWaves * 32);
+    a.q_tiles = (int32_t)tile_count(a.qs, a.nbatch, kWaves * 32);
     a.nblocks = a.q_tiles * a.nsplit * a.heads;
     if (a.nsplit > 1) {
         hipLaunchKernelGGL((attn_kernel<T, D, kWaves, true>), grid_1d(a.nblocks), dim3(kWaves * 64), 0, s, a);
@@ -244,7 +243,7 @@ hipError_t launch_d(AttnArgs a, hipStream_t s) {
 }  // namespace
 
 int attn_splits(const AttnArgs& a) {
-    const int64_t tiles = tile_count(a.q_offsets, a.q_rows, a.nbatch, kWaves * 32) * a.heads;
+    const int64_t tiles = tile_count(a.qs, a.nbatch, kWaves * 32) * a.heads;
     const int64_t cu = device_cu_count();
     const int64_t keys = a.k_rows / a.nbatch;
     int64_t n = cu / (tiles > 0 ? tiles : 1);

@@ -27,9 +27,9 @@ template <typename T> struct HalfRange { static constexpr bool value = false; };
 template <> struct HalfRange<_Float16> { static constexpr bool value = true; };
 
 // Largest of the entries of n rows.
-__device__ __forceinline__ float largest(const float* entries, int64_t n, int lane) {
+__device__ __forceinline__ float largest(const float* entries, int n, int lane) {
     float m = 0.0f;
-    for (int64_t t = lane; t * kPrepRows < n; t += 64) m = fmaxf(m, entries[t]);
+    for (int t = lane; t * kPrepRows < n; t += 64) m = fmaxf(m, entries[t]);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
     return m;
@@ -49,16 +49,17 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
     constexpr int E = D / 16;
     const AttnArgs& f = a.f;
-    const int64_t u = block_linear();
-    if (u >= a.prep_blocks) return;
+    const int64_t p = block_linear();
+    if (p >= a.prep_blocks) return;
+    const int u = (int)p;
     const int m = threadIdx.x & 15, rr = threadIdx.x >> 4;
-    const int64_t qb = a.prep_q_tiles * f.heads;
+    const int qb = a.prep_q_tiles * f.heads;
     __shared__ float top[16];
     float most = 0.0f;
-    int32_t b;
+    int b;
     if (u < qb) {
-        const int head = (int)(u / a.prep_q_tiles);
-        const Rows s = tile_rows<kPrepRows>(f.q_offsets, f.q_rows, f.nbatch, u - head * a.prep_q_tiles, b);
+        const int head = u / a.prep_q_tiles;
+        const Rows s = tile_rows<kPrepRows>(f.qs, f.nbatch, u - head * a.prep_q_tiles, b);
 #pragma unroll
         for (int i = 0; i < kPrepRows / 16; ++i) {
             const int64_t row = s.lo + i * 16 + rr;
@@ -82,10 +83,10 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
             }
         }
     } else {
-        const int64_t w = u - qb;
-        const int head = (int)(w / a.prep_k_tiles);
-        Rows s = tile_rows<kPrepRows>(f.k_offsets, f.k_rows, f.nbatch, w - head * a.prep_k_tiles, b);
-        const int64_t end = segment_keys(f, b).hi;
+        const int w = u - qb;
+        const int head = w / a.prep_k_tiles;
+        Rows s = tile_rows<kPrepRows>(f.ks, f.nbatch, w - head * a.prep_k_tiles, b);
+        const int end = segment_keys(f, b).hi;
         s.hi = end < s.hi ? end : s.hi;
 #pragma unroll
         for (int i = 0; i < kPrepRows / 16; ++i) {
@@ -108,6 +109,9 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
 }
 
 // ---- dk, dv ---------------------------------------------------------------------
+#ifndef T2H_DKV_UNROLL
+#define T2H_DKV_UNROLL 1
+#endif
 constexpr int kQT = 64;   // queries per tile
 
 template <typename T, int D, int NW, int NT, bool SPLIT>
@@ -120,24 +124,24 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a
     const AttnArgs& f = a.f;
     const int64_t p = block_linear();
     if (p >= a.kv_blocks) return;
-    const int64_t u = xcd_order(p, a.kv_blocks);
-    const int64_t per_head = a.k_tiles * a.kv_split;
-    const int kvh = (int)(u / per_head);
-    const int64_t rem = u - kvh * per_head;
-    const int split = (int)(rem / a.k_tiles);
-    int32_t b;
-    const Rows ks = tile_rows<BK>(f.k_offsets, f.k_rows, f.nbatch, rem - split * a.k_tiles, b);
+    const int u = xcd_order((int)p, a.kv_blocks);
+    const int per_head = a.k_tiles * a.kv_split;
+    const int kvh = u / per_head;
+    const int rem = u - kvh * per_head;
+    const int split = SPLIT ? rem / a.k_tiles : 0;
+    int b;
+    const Rows ks = tile_rows<BK>(f.ks, f.nbatch, rem - split * a.k_tiles, b);
     if (ks.lo >= ks.hi) return;
-    const Rows qs = segment_rows(f.q_offsets, f.q_rows, f.nbatch, b);
+    const Rows qs = segment_rows(f.qs, b);
     // keys from k_end on do not count: their gradients are zero
     const Rows seg = segment_keys(f, b);
-    const int64_t k_end = seg.hi;
+    const int k_end = seg.hi;
 
     const int lane = lane_id(), r = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t k0 = ks.lo + wave * (NT * 16);
+    const int k0 = ks.lo + wave * (NT * 16);
     const bool active = k0 < k_end;
-    const int tiles = (int)((qs.hi - qs.lo + kQT - 1) / kQT);
+    const int tiles = (qs.hi - qs.lo + kQT - 1) / kQT;
     const int total = ks.lo < k_end ? tiles * f.group : 0;
     const int it0 = SPLIT ? (int)((int64_t)total * split / a.kv_split) : 0;
     const int it1 = SPLIT ? (int)((int64_t)total * (split + 1) / a.kv_split) : total;
@@ -158,31 +162,39 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a
     if (it0 < it1) {
         if constexpr (kF16) {
             float g2 = 0.0f;
-            const int64_t qt0 = first_tile<kPrepRows>(f.q_offsets, f.q_rows, f.nbatch, b);
+            const int qt0 = first_tile<kPrepRows>(f.qs, b);
             for (int i = 0; i < f.group; ++i)
                 g2 = fmaxf(g2, largest(a.g_most + (kvh * f.group + i) * a.prep_q_tiles + qt0, qs.hi - qs.lo, lane));
-            const int64_t kt0 = first_tile<kPrepRows>(f.k_offsets, f.k_rows, f.nbatch, b);
+            const int kt0 = first_tile<kPrepRows>(f.ks, b);
             shift = shift_ds(g2, largest(a.v_most + kvh * a.prep_k_tiles + kt0, seg.hi - seg.lo, lane));
             z = exp2_f(shift - kShiftP);
         }
-        const auto issue = [&](int it, int st) {
-            const int g = it / tiles;
-            const int head = kvh * f.group + g;
-            const int64_t row = qs.lo + (int64_t)(it - g * tiles) * kQT;
+        // the next tile: query head and first row
+        int head = kvh * f.group, row = qs.lo;
+        if constexpr (SPLIT) {
+            head += it0 / tiles;
+            row += it0 % tiles * kQT;
+        }
+        const auto issue = [&](int st) {
             lq.issue(static_cast<const uint8_t*>(f.q) + head * f.q_head * 2, row, qs.hi, lds + st * kTile);
             lg.issue(static_cast<const uint8_t*>(a.dout) + head * a.do_head * 2, row, qs.hi, lds + (2 + st) * kTile);
             if (wave < 2) {
-                const int64_t at = head * f.q_rows + row, left = qs.hi - row;
-                const float* src = (wave == 0 ? a.lse2 : a.delta) + at;
+                const float* src = (wave == 0 ? a.lse2 : a.delta) + (head * f.q_rows + row);
+                const int left = qs.hi - row;
                 const __amdgpu_buffer_rsrc_t rs = rows_rsrc(reinterpret_cast<const uint8_t*>(src),
                                                             (uint32_t)(left < kQT ? left : kQT) * 4);
                 rsrc_to_lds4(rs, lds + 4 * kTile + (2 * wave + st) * kQT * 4, (uint32_t)lane * 4);
             }
+            row += kQT;
+            if (row >= qs.hi) {
+                row = qs.lo;
+                ++head;
+            }
         };
-        issue(it0, 0);
+        issue(0);
         if (active) {
-            const uint8_t* kb = static_cast<const uint8_t*>(f.k) + (kvh * f.k_head + k0 * f.k_row) * 2;
-            const uint8_t* vb = static_cast<const uint8_t*>(f.v) + (kvh * f.v_head + k0 * f.v_row) * 2;
+            const uint8_t* kb = static_cast<const uint8_t*>(f.k) + (kvh * f.k_head + (int64_t)k0 * f.k_row) * 2;
+            const uint8_t* vb = static_cast<const uint8_t*>(f.v) + (kvh * f.v_head + (int64_t)k0 * f.v_row) * 2;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 load_own<T, D>(k[j], kb + 16 * j * f.k_row * 2, k_end - k0 - 16 * j, (uint32_t)f.k_row * 2, lane);
@@ -194,13 +206,13 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a
             wait_loads<0>();
             wait_lds_reads();
             tile_barrier();
-            if (it + 1 < it1) issue(it + 1, 1 - st);
+            if (it + 1 < it1) issue(1 - st);
             if (!active) continue;
             const uint8_t* qt = lds + st * kTile;
             const uint8_t* gt = lds + (2 + st) * kTile;
             const float* ls = reinterpret_cast<const float*>(lds + 4 * kTile) + st * kQT;
             const float* de = ls + 2 * kQT;
-#pragma unroll
+#pragma unroll T2H_DKV_UNROLL
             for (int s2 = 0; s2 < kQT / 32; ++s2) {
                 f32x4 s[2][NT], d[2][NT];
 #pragma unroll
@@ -260,7 +272,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a
     const float wk = f.scale * (kF16 ? exp2_f(-shift) : 1.0f), wv = kF16 ? exp2_f(-kShiftP) : 1.0f;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        const int64_t row = k0 + 16 * j + r;
+        const int row = k0 + 16 * j + r;
         if (row >= ks.hi) continue;
         const bool counts = row < k_end;
         if constexpr (SPLIT) {
@@ -273,8 +285,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a
                 *reinterpret_cast<f32x4*>(pv + 16 * i) = counts ? dv[i][j] * wv : zero;
             }
         } else {
-            T* pk = static_cast<T*>(a.dk) + row * a.dk_row + kvh * a.dk_head + 4 * h;
-            T* pv = static_cast<T*>(a.dv) + row * a.dv_row + kvh * a.dv_head + 4 * h;
+            T* pk = static_cast<T*>(a.dk) + (int64_t)row * a.dk_row + kvh * a.dk_head + 4 * h;
+            T* pv = static_cast<T*>(a.dv) + (int64_t)row * a.dv_row + kvh * a.dv_head + 4 * h;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 typename AttnMma<T>::v4 x, y;
@@ -303,28 +315,27 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dq_kernel(AttnBwdArgs a)
     const AttnArgs& f = a.f;
     const int64_t p = block_linear();
     if (p >= a.q_blocks) return;
-    const int64_t u = xcd_order(p, a.q_blocks);
-    const int64_t per_head = f.q_tiles * a.q_split;
-    const int head = (int)(u / per_head);
-    const int64_t rem = u - head * per_head;
-    const int split = (int)(rem / f.q_tiles);
-    int32_t b;
-    const Rows qs = tile_rows<BQ>(f.q_offsets, f.q_rows, f.nbatch, rem - split * f.q_tiles, b);
+    const int u = xcd_order((int)p, a.q_blocks);
+    const int per_head = f.q_tiles * a.q_split;
+    const int head = u / per_head;
+    const int rem = u - head * per_head;
+    const int split = SPLIT ? rem / f.q_tiles : 0;
+    int b;
+    const Rows qs = tile_rows<BQ>(f.qs, f.nbatch, rem - split * f.q_tiles, b);
     if (qs.lo >= qs.hi) return;
     Rows ks = segment_keys(f, b);
-    const int64_t keys = ks.hi - ks.lo;
+    const int keys = ks.hi - ks.lo;
     if constexpr (SPLIT) {
-        const int64_t tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
-        const int64_t t0 = tiles * split / a.q_split, t1 = tiles * (split + 1) / a.q_split;
-        const int64_t hi = ks.lo + t1 * kKT;
-        if (hi < ks.hi) ks.hi = hi;
+        const int tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
+        const int t0 = (int)((int64_t)tiles * split / a.q_split), t1 = (int)((int64_t)tiles * (split + 1) / a.q_split);
+        if (t1 < tiles) ks.hi = ks.lo + t1 * kKT;
         ks.lo += t0 * kKT;
     }
-    const int n = (int)((ks.hi - ks.lo + kKT - 1) / kKT);
+    const int n = ks.hi > ks.lo ? (ks.hi - ks.lo + kKT - 1) / kKT : 0;
 
     const int lane = lane_id(), r = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t q0 = qs.lo + wave * (NT * 16);
+    const int q0 = qs.lo + wave * (NT * 16);
     const bool active = q0 < qs.hi;
     const int kvh = head / f.group;
     const uint8_t* kb = static_cast<const uint8_t*>(f.k) + kvh * f.k_head * 2;
@@ -353,14 +364,14 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dq_kernel(AttnBwdArgs a)
         if (active) {
             float v2 = 0.0f;
             if constexpr (kF16)
-                v2 = largest(a.v_most + kvh * a.prep_k_tiles + first_tile<kPrepRows>(f.k_offsets, f.k_rows, f.nbatch, b), keys, lane);
-            const uint8_t* qb = static_cast<const uint8_t*>(f.q) + (head * f.q_head + q0 * f.q_row) * 2;
-            const uint8_t* gb = static_cast<const uint8_t*>(a.dout) + (head * a.do_head + q0 * a.do_row) * 2;
+                v2 = largest(a.v_most + kvh * a.prep_k_tiles + first_tile<kPrepRows>(f.ks, b), keys, lane);
+            const uint8_t* qb = static_cast<const uint8_t*>(f.q) + (head * f.q_head + (int64_t)q0 * f.q_row) * 2;
+            const uint8_t* gb = static_cast<const uint8_t*>(a.dout) + (head * a.do_head + (int64_t)q0 * a.do_row) * 2;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 load_own<T, D>(q[j], qb + 16 * j * f.q_row * 2, qs.hi - q0 - 16 * j, (uint32_t)f.q_row * 2, lane);
                 load_own<T, D>(g[j], gb + 16 * j * a.do_row * 2, qs.hi - q0 - 16 * j, (uint32_t)a.do_row * 2, lane);
-                const int64_t row = q0 + 16 * j + r;
+                const int row = q0 + 16 * j + r;
                 if (row < qs.hi) {
                     l2[j] = a.lse2[head * f.q_rows + row];
                     de[j] = a.delta[head * f.q_rows + row];
@@ -386,11 +397,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dq_kernel(AttnBwdArgs a)
             wait_lds_reads();
             tile_barrier();
             if (t + 1 < n) {
-                lk.issue(kb, ks.lo + (t + 1) * (int64_t)kKT, ks.hi, lds + (1 - st) * kTile);
-                lv.issue(vb, ks.lo + (t + 1) * (int64_t)kKT, ks.hi, lds + (3 - st) * kTile);
+                lk.issue(kb, ks.lo + (t + 1) * kKT, ks.hi, lds + (1 - st) * kTile);
+                lv.issue(vb, ks.lo + (t + 1) * kKT, ks.hi, lds + (3 - st) * kTile);
             }
             if (!active) continue;
-            const int64_t left = ks.hi - ks.lo - t * (int64_t)kKT;
+            const int left = ks.hi - ks.lo - t * kKT;
             const uint8_t* kt = lds + st * kTile;
             const uint8_t* vt = lds + (2 + st) * kTile;
 #pragma unroll
@@ -451,14 +462,14 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dq_kernel(AttnBwdArgs a)
     if (!active) return;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        const int64_t row = q0 + 16 * j + r;
+        const int row = q0 + 16 * j + r;
         if (row >= qs.hi) continue;
         if constexpr (SPLIT) {
             float* po = a.part + (((int64_t)split * f.q_rows + row) * f.heads + head) * D + 4 * h;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(po + 16 * i) = dq[i][j] * w[j];
         } else {
-            T* po = static_cast<T*>(a.dq) + row * a.dq_row + head * a.dq_head + 4 * h;
+            T* po = static_cast<T*>(a.dq) + (int64_t)row * a.dq_row + head * a.dq_head + 4 * h;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 typename AttnMma<T>::v4 x;
@@ -501,7 +512,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(SumArgs a) {
 
 constexpr int kDqWaves = 8, kDqTiles = 2;
 #ifndef T2H_DKV_WAVES
-#define T2H_DKV_WAVES 4
+#define T2H_DKV_WAVES 8
 #define T2H_DKV_TILES 2
 #endif
 constexpr int kDkvWaves = T2H_DKV_WAVES, kDkvTiles = T2H_DKV_TILES;
@@ -511,7 +522,7 @@ template <typename T, int D>
 hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
     AttnArgs& f = a.f;
     if (a.prep_blocks > 0) hipLaunchKernelGGL((attn_prep_kernel<T, D>), grid_1d(a.prep_blocks), dim3(256), 0, s, a);
-    a.k_tiles = tile_count(f.k_offsets, f.k_rows, f.nbatch, kBK);
+    a.k_tiles = (int32_t)tile_count(f.ks, f.nbatch, kBK);
     a.kv_blocks = a.k_tiles * a.kv_split * a.kv_heads;
     if (a.kv_blocks > 0) {
         if (a.kv_split > 1) {
@@ -525,7 +536,7 @@ hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
             m.row_stride[1] = a.dv_row;
             m.head_stride[0] = a.dk_head;
             m.head_stride[1] = a.dv_head;
-            m.offsets = f.k_offsets;
+            m.offsets = f.ks.offsets;
             m.rows = f.k_rows;
             m.heads = a.kv_heads;
             m.nsplit = a.kv_split;
@@ -537,7 +548,7 @@ hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
             hipLaunchKernelGGL((attn_dkv_kernel<T, D, kDkvWaves, kDkvTiles, false>), grid_1d(a.kv_blocks), dim3(kDkvWaves * 64), 0, s, a);
         }
     }
-    f.q_tiles = tile_count(f.q_offsets, f.q_rows, f.nbatch, kBQ);
+    f.q_tiles = (int32_t)tile_count(f.qs, f.nbatch, kBQ);
     a.q_blocks = f.q_tiles * a.q_split * f.heads;
     if (a.q_blocks > 0) {
         if (a.q_split > 1) {
@@ -547,7 +558,7 @@ hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
             m.out[0] = a.dq;
             m.row_stride[0] = a.dq_row;
             m.head_stride[0] = a.dq_head;
-            m.offsets = f.q_offsets;
+            m.offsets = f.qs.offsets;
             m.rows = f.q_rows;
             m.heads = f.heads;
             m.nsplit = a.q_split;
@@ -574,8 +585,8 @@ int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 // parts of whichever of dk, dv and dq are split (one after the other).
 int64_t attn_bwd_plan(AttnBwdArgs& a, void* workspace) {
     AttnArgs& f = a.f;
-    a.prep_q_tiles = tile_count(f.q_offsets, f.q_rows, f.nbatch, kPrepRows);
-    a.prep_k_tiles = tile_count(f.k_offsets, f.k_rows, f.nbatch, kPrepRows);
+    a.prep_q_tiles = (int32_t)tile_count(f.qs, f.nbatch, kPrepRows);
+    a.prep_k_tiles = (int32_t)tile_count(f.ks, f.nbatch, kPrepRows);
     a.prep_blocks = a.prep_q_tiles * f.heads + (f.dtype == T2H_F16 ? a.prep_k_tiles * a.kv_heads : 0);
     const int64_t kt = (f.k_rows / f.nbatch + kBK - 1) / kBK * f.nbatch, qt = (f.q_rows / f.nbatch + kBQ - 1) / kBQ * f.nbatch;
     a.kv_split = splits(kt * a.kv_heads, f.q_rows / f.nbatch * f.group, 2 * kQT);

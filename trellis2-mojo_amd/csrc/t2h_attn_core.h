@@ -65,77 +65,72 @@ __device__ __forceinline__ void wait_loads() {
 __device__ __forceinline__ void wait_lds_reads() { __builtin_amdgcn_s_waitcnt(0xC07F); }   // lgkmcnt(0)
 
 // ---- segments ---------------------------------------------------------------
-// Rows [lo, hi) of segment b: from the offsets, kept inside the tensor whatever
-// they are, or equal shares.
-struct Rows { int64_t lo, hi; };
-__device__ __forceinline__ int64_t offset_at(const int64_t* offsets, int64_t rows, int32_t b) {
+// Row numbers are 32-bit (the entry points take no more rows); addresses are not.
+struct Rows { int lo, hi; };
+// Offset b, kept inside the tensor whatever it is.
+__device__ __forceinline__ int offset_at(const int64_t* offsets, int rows, int b) {
     const int64_t o = offsets[b];
-    return o < 0 ? 0 : o > rows ? rows : o;
+    return o < 0 ? 0 : o > rows ? rows : (int)o;
 }
-__device__ __forceinline__ Rows segment_rows(const int64_t* offsets, int64_t rows, int32_t nbatch, int32_t b) {
+// Rows [lo, hi) of segment b: from the offsets, or equal shares.
+__device__ __forceinline__ Rows segment_rows(const AttnSide& a, int b) {
     Rows s;
-    if (offsets != nullptr) {
-        s.lo = offset_at(offsets, rows, b);
-        s.hi = offset_at(offsets, rows, b + 1);
+    if (a.offsets != nullptr) {
+        s.lo = offset_at(a.offsets, a.rows, b);
+        s.hi = offset_at(a.offsets, a.rows, b + 1);
         s.hi = s.hi < s.lo ? s.lo : s.hi;
     } else {
-        const int64_t n = rows / nbatch;
-        s.lo = b * n;
-        s.hi = s.lo + n;
+        s.lo = b * a.share;
+        s.hi = s.lo + a.share;
+    }
+    return s;
+}
+// ... those of its keys that count.
+__device__ __forceinline__ Rows segment_keys(const AttnArgs& a, int b) {
+    Rows s = segment_rows(a.ks, b);
+    if (a.k_lens != nullptr) {
+        const int64_t n = a.k_lens[b] < 0 ? 0 : a.k_lens[b];
+        if (n < s.hi - s.lo) s.hi = s.lo + (int)n;
     }
     return s;
 }
 
-// Tile t of a ragged side: segment b's tiles have the numbers from
-// offsets[b] / BT + b on, which leaves room for ceil(length / BT) of them, so a
-// tile's segment is found by bisection and no prefix sum of tile counts is
-// needed. Numbers that no tile has come back with lo >= hi.
+// Number of segment b's first tile of BT rows: offsets[b] / BT + b, which leaves
+// room for the ceil(length / BT) tiles of each segment, so a tile's segment is
+// found by bisection and no prefix sum of tile counts is needed.
 template <int BT>
-__device__ __forceinline__ Rows tile_rows(const int64_t* offsets, int64_t rows, int32_t nbatch, int64_t t, int32_t& b) {
-    Rows s;
-    if (offsets != nullptr) {
-        int32_t lo = 0, hi = nbatch - 1;
+__device__ __forceinline__ int first_tile(const AttnSide& a, int b) {
+    return a.offsets != nullptr ? offset_at(a.offsets, a.rows, b) / BT + b : (a.share + BT - 1) / BT * b;
+}
+// Rows of tile t and its segment b; a number that no tile has comes back with lo >= hi.
+template <int BT>
+__device__ __forceinline__ Rows tile_rows(const AttnSide& a, int nbatch, int t, int& b) {
+    if (a.offsets != nullptr) {
+        int lo = 0, hi = nbatch - 1;
         while (lo < hi) {
-            const int32_t mid = (lo + hi + 1) >> 1;
-            if (offset_at(offsets, rows, mid) / BT + mid <= t) lo = mid; else hi = mid - 1;
+            const int mid = (lo + hi + 1) >> 1;
+            if (first_tile<BT>(a, mid) <= t) lo = mid; else hi = mid - 1;
         }
         b = lo;
-        s = segment_rows(offsets, rows, nbatch, b);
-        const int64_t i = t - (offset_at(offsets, rows, b) / BT + b);
-        s.lo = i < 0 ? s.hi : s.lo + i * BT;
     } else {
-        const int64_t n = rows / nbatch, per = (n + BT - 1) / BT;
-        b = (int32_t)(t / per);
-        s.lo = b * n + (t - b * per) * BT;
-        s.hi = (b + 1) * n;
+        b = t / ((a.share + BT - 1) / BT);
     }
+    Rows s = segment_rows(a, b);
+    const int i = t - first_tile<BT>(a, b);
+    s.lo = i < 0 || i > (s.hi - s.lo) / BT ? s.hi : s.lo + i * BT;
     return s;
 }
-// Number of segment b's first tile.
-template <int BT>
-__device__ __forceinline__ int64_t first_tile(const int64_t* offsets, int64_t rows, int32_t nbatch, int32_t b) {
-    return offsets != nullptr ? offset_at(offsets, rows, b) / BT + b : (rows / nbatch + BT - 1) / BT * b;
-}
-// Rows of segment b's keys that count.
-__device__ __forceinline__ Rows segment_keys(const AttnArgs& a, int32_t b) {
-    Rows s = segment_rows(a.k_offsets, a.k_rows, a.nbatch, b);
-    if (a.k_lens != nullptr) {
-        const int64_t n = a.k_lens[b] < 0 ? 0 : a.k_lens[b];
-        if (n < s.hi - s.lo) s.hi = s.lo + n;
-    }
-    return s;
-}
-// Tiles that tile_rows() numbers (host).
-inline int64_t tile_count(const int64_t* offsets, int64_t rows, int32_t nbatch, int bt) {
-    if (offsets != nullptr) return rows / bt + nbatch;
-    return (rows / nbatch + bt - 1) / bt * nbatch;
+// Tile numbers of a side (host).
+inline int64_t tile_count(const AttnSide& a, int32_t nbatch, int bt) {
+    if (a.offsets != nullptr) return a.rows / bt + nbatch;
+    return (int64_t)((a.share + (int64_t)bt - 1) / bt) * nbatch;
 }
 
 // Logical number of physical block p of nb: contiguous ranges for the 8 XCDs
 // (block p runs on XCD p % 8), so that the blocks one L2 serves at a time share
 // a head's streaming side.
-__device__ __forceinline__ int64_t xcd_order(int64_t p, int64_t nb) {
-    const int64_t x = p & 7, i = p >> 3, q = nb >> 3, r = nb & 7;
+__device__ __forceinline__ int xcd_order(int p, int nb) {
+    const int x = p & 7, i = p >> 3, q = nb >> 3, r = nb & 7;
     return x * q + (x < r ? x : r) + i;
 }
 
@@ -151,8 +146,8 @@ __device__ __forceinline__ int swizzle(int t) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (int)bytes, 0x00020000);
 }
-__device__ __forceinline__ void rsrc_to_lds16(__amdgpu_buffer_rsrc_t r, uint8_t* lds, uint32_t off) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)off, 0, 0, 0);
+__device__ __forceinline__ void rsrc_to_lds16(__amdgpu_buffer_rsrc_t r, uint8_t* lds, uint32_t off, uint32_t soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)off, (int)soff, 0, 0);
 }
 __device__ __forceinline__ void rsrc_to_lds4(__amdgpu_buffer_rsrc_t r, uint8_t* lds, uint32_t off) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 4, (int)off, 0, 0, 0);
@@ -171,8 +166,8 @@ __device__ __forceinline__ s16x4 lds_read_tr(const uint8_t* __restrict p) {
 // Bytes that a resource over n rows (at most BT) of 2 D bytes, stride bytes
 // apart, covers: loads of rows past them return zeros, whatever memory holds there.
 template <int D, int BT>
-__device__ __forceinline__ uint32_t span_bytes(int64_t n, uint32_t stride) {
-    const int m = n < BT ? (n < 0 ? 0 : (int)n) : BT;
+__device__ __forceinline__ uint32_t span_bytes(int n, uint32_t stride) {
+    const int m = n < BT ? (n < 0 ? 0 : n) : BT;
     return m > 0 ? (uint32_t)(m - 1) * stride + D * 2 : 0;
 }
 
@@ -182,7 +177,7 @@ template <int D, int BT, int NW> struct TileLoad {
     static constexpr int kRowsPer = 512 / D;                 // rows of one wave's KB
     static constexpr int kLoads = kBytes / 1024 / NW;        // per wave
     static_assert(kBytes % (1024 * NW) == 0 && (kRowsPer * NW) % 16 == 0, "tile and waves");
-    uint32_t off, stride, step;
+    uint32_t off, stride;
     int wave;
     __device__ __forceinline__ void init(int wave_, int lane, int64_t row_stride) {
         wave = wave_;
@@ -190,13 +185,13 @@ template <int D, int BT, int NW> struct TileLoad {
         constexpr int kChunks = D / 8;
         const int t = wave * kRowsPer + lane / kChunks;
         off = (uint32_t)t * stride + (uint32_t)((lane % kChunks) ^ swizzle<D>(t & 15)) * 16;
-        step = (uint32_t)(kRowsPer * NW) * stride;
     }
     // rows [row, row + BT) of the tensor at base, those from hi on as zeros
-    __device__ __forceinline__ void issue(const uint8_t* base, int64_t row, int64_t hi, uint8_t* lds) const {
-        const __amdgpu_buffer_rsrc_t r = rows_rsrc(base + row * stride, span_bytes<D, BT>(hi - row, stride));
+    __device__ __forceinline__ void issue(const uint8_t* base, int row, int hi, uint8_t* lds) const {
+        const __amdgpu_buffer_rsrc_t r = rows_rsrc(base + (int64_t)row * stride, span_bytes<D, BT>(hi - row, stride));
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) rsrc_to_lds16(r, lds + (i * NW + wave) * 1024, off + i * step);
+        for (int i = 0; i < kLoads; ++i)
+            rsrc_to_lds16(r, lds + (i * NW + wave) * 1024, off, (uint32_t)(i * kRowsPer * NW) * stride);
     }
 };
 
@@ -228,7 +223,7 @@ __device__ __forceinline__ typename AttnMma<T>::v8 tr_frag(const uint8_t* tile, 
 // A wave's own 16-token operand tile as B fragments, from memory: token r,
 // elements 32 s + 8 h ..; tokens past n as zeros.
 template <typename T, int D>
-__device__ __forceinline__ void load_own(typename AttnMma<T>::v8 (&f)[D / 32], const uint8_t* base, int64_t n,
+__device__ __forceinline__ void load_own(typename AttnMma<T>::v8 (&f)[D / 32], const uint8_t* base, int n,
                                          uint32_t stride, int lane) {
     const __amdgpu_buffer_rsrc_t r = rows_rsrc(base, span_bytes<D, 16>(n, stride));
     const uint32_t off = (uint32_t)(lane & 15) * stride + (uint32_t)(lane >> 4) * 16;
