@@ -29,15 +29,42 @@ __device__ __forceinline__ float head_sum(float v) {
     else return row8_sum(v);
 }
 
+// One row's pieces of a wave, as loaded: the next row's are in flight while this
+// one is worked on.
+template <typename T, int D, int NG, int LPH> struct RowPieces {
+    using L = HeadLanes<T, D, LPH>;
+    static constexpr int HPI = 64 / LPH;
+    static constexpr int kWords = L::VE * (int)sizeof(T) / 4;   // 4, or 2 (f32 of head_dim 64 has 4 too)
+    typedef uint32_t W __attribute__((ext_vector_type(kWords)));
+    W w[NG][L::NC];
+    __device__ __forceinline__ void load(const T* row, int H, int g, int m) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int hh = HPI * i + g < H ? HPI * i + g : H - 1;
+#pragma unroll
+            for (int j = 0; j < L::NC; ++j)
+                w[i][j] = __builtin_nontemporal_load(reinterpret_cast<const W*>(row + (int64_t)hh * D + L::piece(m, j)));
+        }
+    }
+    __device__ __forceinline__ void get(int i, float* f) const {
+#pragma unroll
+        for (int j = 0; j < L::NC; ++j)
+#pragma unroll
+            for (int c = 0; c < kWords; ++c) Word<T>::unpack(w[i][j][c], f + j * L::VE + c * Word<T>::N);
+    }
+};
+
 // Head layout as the forward's (HeadLanes): LPH lanes per head, NG groups of
 // 64 / LPH heads.
 template <typename T, int D, int NG>
-__global__ __launch_bounds__(kW * 64) void qk_bwd_kernel(QkBwdArgs a, RopeSlots tab) {
+__global__ __launch_bounds__(kW * 64, sizeof(T) == 2 && NG < 4 ? 3 : 2) void qk_bwd_kernel(QkBwdArgs a, RopeSlots tab) {
     constexpr int LPH = (sizeof(T) == 2 && D == 64) ? 8 : 16;
     constexpr int HPI = 64 / LPH;
     using L = HeadLanes<T, D, LPH>;
+    using Pieces = RowPieces<T, D, NG, LPH>;
     constexpr int E = L::E, P = L::P, HALF = D / 2;
-    __shared__ __attribute__((aligned(16))) float sums[kW][NG * HPI * D];
+    // gamma * scale and bias while rows are worked on, the waves' sums afterwards
+    __shared__ __attribute__((aligned(16))) float lds[kW][NG * HPI * D];
     const int lane = lane_id(), g = lane / LPH, m = lane % LPH;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int H = a.heads, HD = H * D;
@@ -47,84 +74,96 @@ __global__ __launch_bounds__(kW * 64) void qk_bwd_kernel(QkBwdArgs a, RopeSlots 
     const T* __restrict__ x = static_cast<const T*>(t.x);
     const T* __restrict__ dy = static_cast<const T*>(t.dy);
     T* __restrict__ dx = static_cast<T*>(t.dx);
-    const bool norm = t.gamma != nullptr;
+    const bool norm = t.gamma != nullptr, biased = norm && t.bias != nullptr;
+    const bool turn = a.use_rope && a.phases == nullptr;
     const PosSource src{a.coords, a.coord_cols, a.grid_res, a.pos_dim};
     const int my_slot = lane % HALF;
-    const int my_axis = slot_axis(my_slot, a.freq_dim, a.pos_dim);
+    const int my_axis = turn ? slot_axis(my_slot, a.freq_dim, a.pos_dim) : -1;
     const float my_freq = tab.freq[my_slot];
+    const int64_t step = a.blocks * kW;
 
-    float gm[NG][E], bs[NG][E], sg[NG][E], sb[NG][E];
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        const int hh = HPI * i + g < H ? HPI * i + g : H - 1;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            gm[i][e] = 1.0f;
-            bs[i][e] = sg[i][e] = sb[i][e] = 0.0f;
-        }
-        if (norm) {
-            L::params(t.gamma + hh * D, m, gm[i]);
-#pragma unroll
-            for (int e = 0; e < E; ++e) gm[i][e] *= a.rms_scale;
-        }
-        if (t.bias != nullptr) L::params(t.bias + hh * D, m, bs[i]);
+    int64_t r = blk * kW + wave;
+    Pieces xn, gn;
+    int pos = 0;
+    if (r < a.rows) {
+        if (my_axis >= 0) pos = src.at(r, my_axis);
+        gn.load(dy + r * a.dy_stride, H, g, m);
+        if (norm) xn.load(x + r * a.x_stride, H, g, m);
     }
-    for (int64_t r = blk * kW + wave; r < a.rows; r += a.blocks * kW) {
-        float xv[NG][E], gv[NG][E];
+    if (norm)
+        for (int c = threadIdx.x; c < HD; c += kW * 64) {
+            lds[0][c] = t.gamma[c] * a.rms_scale;
+            if (biased) lds[1][c] = t.bias[c];
+        }
+    __syncthreads();
+    float sg[NG][E], sb[NG][E];
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int hh = HPI * i + g < H ? HPI * i + g : H - 1;
-            L::load(dy + r * a.dy_stride + (int64_t)hh * D, m, gv[i]);
-            if (norm) L::load(x + r * a.x_stride + (int64_t)hh * D, m, xv[i]);
+    for (int i = 0; i < NG; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) sg[i][e] = sb[i][e] = 0.0f;
+    for (; r < a.rows; r += step) {
+        const Pieces xr = xn, gr = gn;
+        const int at = pos;
+        if (r + step < a.rows) {
+            if (my_axis >= 0) pos = src.at(r + step, my_axis);
+            gn.load(dy + (r + step) * a.dy_stride, H, g, m);
+            if (norm) xn.load(x + (r + step) * a.x_stride, H, g, m);
         }
         float pc[P], ps[P];
-        if (a.use_rope) {
-            if (a.phases != nullptr) {
-                L::phases(a.phases + r % a.phase_rows * (HALF * 2), m, pc, ps);
-            } else {
-                float c = 1.0f, s = 0.0f;
-                if (my_axis >= 0) sincosf(mul_rn((float)src.at(r, my_axis), my_freq), &s, &c);
+        if (turn) {
+            float c = 1.0f, s = 0.0f;
+            if (my_axis >= 0) sincosf(mul_rn((float)at, my_freq), &s, &c);
 #pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    pc[p] = lane_bcast(c, L::slot(m, p));
-                    ps[p] = lane_bcast(s, L::slot(m, p));
-                }
+            for (int p = 0; p < P; ++p) {
+                pc[p] = lane_bcast(c, L::slot(m, p));
+                ps[p] = lane_bcast(s, L::slot(m, p));
             }
+        } else if (a.use_rope) {
+            L::phases(a.phases + r % a.phase_rows * (HALF * 2), m, pc, ps);
         }
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             const bool valid = HPI * i + g < H;
+            const int hl = valid ? HPI * i + g : H - 1;
+            float gv[E];
+            gr.get(i, gv);
             if (a.use_rope) {
 #pragma unroll
-                for (int p = 0; p < P; ++p) rotate_pair(gv[i][2 * p], gv[i][2 * p + 1], pc[p], -ps[p]);
+                for (int p = 0; p < P; ++p) rotate_pair(gv[2 * p], gv[2 * p + 1], pc[p], -ps[p]);
             }
             if (norm) {
+                float xv[E], gm[E];
+                xr.get(i, xv);
+                if (biased) {
+                    float bs[E];
+                    L::params(&lds[1][hl * D], m, bs);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) xv[e] = add_rn(xv[e], bs[e]);
+                }
+                L::params(&lds[0][hl * D], m, gm);
                 float ss = 0.0f, dot = 0.0f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    xv[i][e] = add_rn(xv[i][e], bs[i][e]);
-                    ss = fmaf(xv[i][e], xv[i][e], ss);
-                }
+                for (int e = 0; e < E; ++e) ss = fmaf(xv[e], xv[e], ss);
                 ss = head_sum<LPH>(ss);
                 const bool floor = ss < 1e-24f;
                 const float rn = floor ? 1e12f : __builtin_amdgcn_rsqf(ss);
-                float w[E];
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    xv[i][e] *= rn;
-                    w[e] = gv[i][e] * gm[i][e];
-                    dot = fmaf(w[e], xv[i][e], dot);
-                    sg[i][e] = fmaf(gv[i][e], xv[i][e], sg[i][e]);
+                    xv[e] *= rn;
+                    sg[i][e] = fmaf(gv[e], xv[e], sg[i][e]);
+                    gv[e] *= gm[e];
+                    dot = fmaf(gv[e], xv[e], dot);
                 }
                 dot = floor ? 0.0f : head_sum<LPH>(dot);
 #pragma unroll
-                for (int e = 0; e < E; ++e) gv[i][e] = fmaf(-xv[i][e], dot, w[e]) * rn;
+                for (int e = 0; e < E; ++e) gv[e] = fmaf(-xv[e], dot, gv[e]) * rn;
             }
 #pragma unroll
-            for (int e = 0; e < E; ++e) sb[i][e] += gv[i][e];
-            if (valid) L::store(dx + r * a.dx_stride + (int64_t)(HPI * i + g) * D, m, gv[i]);
+            for (int e = 0; e < E; ++e) sb[i][e] += gv[e];
+            if (valid) L::store(dx + r * a.dx_stride + (int64_t)hl * D, m, gv);
         }
     }
+    __syncthreads();
     // the waves' sums joined: dgamma, then dbias
     float* part = a.part + ((int64_t)which * a.blocks + blk) * 2 * HD;
 #pragma unroll
@@ -134,13 +173,13 @@ __global__ __launch_bounds__(kW * 64) void qk_bwd_kernel(QkBwdArgs a, RopeSlots 
         for (int i = 0; i < NG; ++i)
             if (HPI * i + g < H) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) sums[wave][(HPI * i + g) * D + L::elem(m, e)] = k == 0 ? sg[i][e] : sb[i][e];
+                for (int e = 0; e < E; ++e) lds[wave][(HPI * i + g) * D + L::elem(m, e)] = k == 0 ? sg[i][e] : sb[i][e];
             }
         __syncthreads();
         for (int c = threadIdx.x; c < HD; c += kW * 64) {
-            float s = sums[0][c];
+            float s = lds[0][c];
 #pragma unroll
-            for (int w = 1; w < kW; ++w) s += sums[w][c];
+            for (int w = 1; w < kW; ++w) s += lds[w][c];
             part[k * HD + c] = s;
         }
         __syncthreads();
@@ -244,31 +283,35 @@ __global__ __launch_bounds__(kW * 64) void qk_bwd_generic(QkBwdArgs a, RopeSlots
     }
 }
 
-// dgamma and dbias from the partial rows: 64 columns per block, 4 strands of
+// dgamma and dbias from the partial rows: 64 columns per block, 16 strands of
 // partial rows, joined in a fixed order.
-__global__ __launch_bounds__(256) void qk_bwd_sums(QkBwdArgs a) {
-    __shared__ float s[4][64];
+__global__ __launch_bounds__(1024) void qk_bwd_sums(QkBwdArgs a) {
+    __shared__ float s[16][64];
     const int HD = a.heads * a.head_dim;
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), strand = threadIdx.x >> 6;
+    const int c = threadIdx.x & 63, strand = threadIdx.x >> 6;
+    const int col = blockIdx.x * 64 + c;
     const int which = blockIdx.y >> 1, k = blockIdx.y & 1;
     float* out = k == 0 ? a.t[which].dgamma : a.t[which].dbias;
     if (out == nullptr) return;
     float v = 0.0f;
     if (col < HD) {
         const float* part = a.part + ((int64_t)which * a.blocks * 2 + k) * HD + col;
-        for (int64_t b = strand; b < a.blocks; b += 4) v += part[b * 2 * HD];
+#pragma unroll 8
+        for (int64_t b = strand; b < a.blocks; b += 16) v += part[b * 2 * HD];
     }
-    s[strand][threadIdx.x & 63] = v;
+    s[strand][c] = v;
     __syncthreads();
     if (strand == 0 && col < HD) {
-        v = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) v += s[i][c];
         out[col] = k == 0 ? v * a.rms_scale : v;
     }
 }
 
-// Blocks (partial rows) per tensor: two blocks a CU over both tensors.
-int64_t blocks_for(int64_t rows) {
-    const int64_t most = device_cu_count(), need = (rows + kW - 1) / kW;
+// Blocks (partial rows) per tensor: what the CUs hold at once, 3 each, 2 for f32
+// rows (per_cu).
+int64_t blocks_for(int64_t rows, int tensors, int per_cu) {
+    const int64_t most = (int64_t)device_cu_count() * per_cu / tensors, need = (rows + kW - 1) / kW;
     return need < most ? need : most;
 }
 
@@ -316,18 +359,18 @@ hipError_t launch_typed(const QkBwdArgs& a, const RopeSlots& tab, hipStream_t s)
     bool sums = false;
     for (int i = 0; i < a.tensors; ++i) sums |= a.t[i].dgamma != nullptr || a.t[i].dbias != nullptr;
     if (sums)
-        hipLaunchKernelGGL(qk_bwd_sums, dim3((unsigned)((a.heads * a.head_dim + 63) / 64), (unsigned)(2 * a.tensors)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(qk_bwd_sums, dim3((unsigned)((a.heads * a.head_dim + 63) / 64), (unsigned)(2 * a.tensors)), dim3(1024), 0, s, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t qk_bwd_bytes(int64_t rows, int32_t heads, int32_t head_dim, int32_t tensors) {
-    return blocks_for(rows) * tensors * 2 * heads * head_dim * 4;
+    return blocks_for(rows, tensors, 3) * tensors * 2 * heads * head_dim * 4;
 }
 
 hipError_t launch_qk_bwd(QkBwdArgs a, const RopeSlots& tab, hipStream_t s) {
-    a.blocks = blocks_for(a.rows);
+    a.blocks = blocks_for(a.rows, a.tensors, a.dtype == T2H_F32 ? 2 : 3);
     switch (a.dtype) {
         case T2H_F32: return launch_typed<float>(a, tab, s);
         case T2H_F16: return launch_typed<_Float16>(a, tab, s);
