@@ -2,112 +2,125 @@
 //
 //   s_ij = scale * sum_d q_id k_jd       lse_i = log sum_j exp(s_ij)
 //   out_i = sum_j exp(s_ij - lse_i) v_j
+#include <type_traits>
+
 #include "t2h_attn_core.h"
 
 namespace t2h {
 namespace {
 
-constexpr int kKT = 64;   // keys per tile
-
+// A block takes BQ = NW * NT * 16 queries of one head; wave w of the NW * KG
+// keeps NT * 16 of them in registers, as B operands, with the output that its
+// share of the keys gives: of every KG * KT keys that come to LDS (two slots)
+// group w / NW takes KT. The groups' outputs are joined in LDS at the end.
 // The scores are kept unscaled; with c = scale * log2(e), p = exp2(c s - mc), mc
 // = c * (a reference close to the row's running maximum).
-template <typename T, int D, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
+template <typename T, int D, int NW, int NT, int KT, int KG, bool SPLIT>
+__global__ __launch_bounds__(NW * KG * 64, 2) void attn_kernel(AttnArgs a) {
     using V8 = typename AttnMma<T>::v8;
-    constexpr int BQ = NW * 32;
-    constexpr int kTile = kKT * D * 2;
+    constexpr int BQ = NW * NT * 16, BK = KG * KT, kS = KT / 16, kP = KT / 32;
+    constexpr int kTile = KT * D * 2, kStage = KG * kTile;
     constexpr float kRise = 8.0f;   // the reference follows the maximum once it is this far above (log2)
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];   // K, K, V, V
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kStage];   // K, K, V, V
     const int64_t p = block_linear();
     if (p >= a.nblocks) return;
+    const int lane = lane_id(), r = lane & 15, h = lane >> 4;
     const int u = xcd_order((int)p, a.nblocks);
     const int per_head = a.q_tiles * a.nsplit;
     const int head = u / per_head;
     const int rem = u - head * per_head;
     const int split = SPLIT ? rem / a.q_tiles : 0;
     int b;
-    const Rows qs = tile_rows<BQ>(a.qs, a.nbatch, rem - split * a.q_tiles, b);
+    const Rows qs = tile_rows<BQ>(a.qs, a.nbatch, rem - split * a.q_tiles, lane, b);
     if (qs.lo >= qs.hi) return;
     Rows ks = segment_keys(a, b);
     if constexpr (SPLIT) {
-        const int tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
+        const int tiles = (ks.hi - ks.lo + KT - 1) / KT;
         const int t0 = (int)((int64_t)tiles * split / a.nsplit), t1 = (int)((int64_t)tiles * (split + 1) / a.nsplit);
-        if (t1 < tiles) ks.hi = ks.lo + t1 * kKT;
-        ks.lo += t0 * kKT;
+        if (t1 < tiles) ks.hi = ks.lo + t1 * KT;
+        ks.lo += t0 * KT;
     }
-    const int n = ks.hi > ks.lo ? (ks.hi - ks.lo + kKT - 1) / kKT : 0;
+    const int n = ks.hi > ks.lo ? (ks.hi - ks.lo + BK - 1) / BK : 0;
 
-    const int lane = lane_id(), r = lane & 15, h = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int q0 = qs.lo + wave * 32;
+    const int qw = KG == 1 ? wave : wave % NW, kg = KG == 1 ? 0 : wave / NW;
+    const int q0 = qs.lo + qw * (NT * 16);
     const bool active = q0 < qs.hi;
     const int kvh = head / a.group;
     const uint8_t* kb = static_cast<const uint8_t*>(a.k) + kvh * a.k_head * 2;
     const uint8_t* vb = static_cast<const uint8_t*>(a.v) + kvh * a.v_head * 2;
-    TileLoad<D, kKT, NW> lk, lv;
+    TileLoad<D, BK, NW * KG> lk, lv;
     lk.init(wave, lane, a.k_row);
     lv.init(wave, lane, a.v_row);
     const FragAddr<D> fa(lane);
 
-    V8 q[2][D / 32];
-    f32x4 o[D / 16][2];
-    float mc[2] = {0.0f, 0.0f}, thr[2], l[2] = {0.0f, 0.0f};
-    thr[0] = thr[1] = -INFINITY;
+    V8 q[NT][D / 32];
+    f32x4 o[D / 16][NT];
+    float mc[NT], thr[NT], l[NT];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < NT; ++j) {
+        mc[j] = l[j] = 0.0f;
+        thr[j] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     const float c = a.scale * kLog2e;
 
     if (n > 0) {
-        lk.issue(kb, ks.lo, ks.hi, lds);
+        // q and the first tiles; K's second is fetched as zeros where there is none
         if (active) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < NT; ++j)
                 load_own<T, D>(q[j], static_cast<const uint8_t*>(a.q) + head * a.q_head * 2 + (int64_t)(q0 + 16 * j) * a.q_row * 2,
                                qs.hi - q0 - 16 * j, (uint32_t)a.q_row * 2, lane);
         }
-        wait_loads<0>();
+        lk.issue(kb, ks.lo, ks.hi, lds);
+        lv.issue(vb, ks.lo, ks.hi, lds + 2 * kStage);
+        lk.issue(kb, ks.lo + BK, ks.hi, lds + kStage);
+        wait_loads<2 * decltype(lk)::kLoads>();
         tile_barrier();
-        lv.issue(vb, ks.lo, ks.hi, lds + 2 * kTile);
-        if (n > 1) lk.issue(kb, ks.lo + kKT, ks.hi, lds + kTile);
-        f32x4 s[4][2];
-        const auto scores = [&](const uint8_t* kt, f32x4 (&x)[4][2]) {
+        f32x4 sa[kS][NT], sb[kS][NT];
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        const auto scores = [&](const uint8_t* kt, f32x4 (&x)[kS][NT]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i][0] = x[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < kS; ++i)
 #pragma unroll
-            for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int t = 0; t < D / 32; ++t) {
                     const V8 f = row_frag<T, D>(kt, fa.row, i, t);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) x[i][j] = AttnMma<T>::run(f, q[j][t], x[i][j]);
+                    for (int j = 0; j < NT; ++j) x[i][j] = AttnMma<T>::run(f, q[j][t], t == 0 ? zero : x[i][j]);
                 }
         };
         // keys from `left` on do not count
-        const auto mask = [&](f32x4 (&x)[4][2], int left) {
+        const auto mask = [&](f32x4 (&x)[kS][NT], int left) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < kS; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (16 * i + 4 * h + e >= left) x[i][0][e] = x[i][1][e] = -INFINITY;
-        };
-        const auto follow = [&](const f32x4 (&x)[4][2]) {
-            float top[2];
-            bool rise = false;
+                    if (16 * i + 4 * h + e >= left) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+                        for (int j = 0; j < NT; ++j) x[i][j][e] = -INFINITY;
+                    }
+        };
+        const auto tops = [&](const f32x4 (&x)[kS][NT], float (&top)[NT]) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
                 top[j] = x[0][j][0];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < kS; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top[j] = fmaxf(top[j], x[i][j][e]);
-                top[j] *= c;
-                rise |= top[j] > thr[j];
             }
+        };
+        const auto follow = [&](float (&top)[NT]) {
+            bool rise = false;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) rise |= top[j] * c > thr[j];
             if (__any(rise)) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < NT; ++j) {
                     float t = fmaxf(top[j], __shfl_xor(top[j], 16));
-                    t = fmaxf(t, __shfl_xor(t, 32));
+                    t = fmaxf(t, __shfl_xor(t, 32)) * c;
                     if (t > thr[j]) {
                         const float alpha = thr[j] == -INFINITY ? 0.0f : exp2_f(mc[j] - t);
                         mc[j] = t;
@@ -119,26 +132,31 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
                 }
             }
         };
+        float top[NT];
+        const int mine = ks.hi - ks.lo - kg * KT;      // keys from the group's first on
         if (active) {
-            scores(lds, s);
-            if (n == 1) mask(s, ks.hi - ks.lo);
-            follow(s);
+            scores(lds + kg * kTile, sa);
+            if (mine < KT) mask(sa, mine);
+            tops(sa, top);
+            follow(top);
         }
-        for (int t = 0; t < n; ++t) {
+        // Tile t: its probabilities from s while the matrix cores make the next
+        // tile's scores (MORE), then its part of the output.
+        const auto tile = [&](auto more, int t, f32x4 (&s)[kS][NT], f32x4 (&sn)[kS][NT]) {
+            constexpr bool MORE = decltype(more)::value;
             wait_loads<0>();
             wait_lds_reads();
             tile_barrier();
             const int st = t & 1;
-            if (t + 1 < n) lv.issue(vb, ks.lo + (t + 1) * kKT, ks.hi, lds + (3 - st) * kTile);
-            if (t + 2 < n) lk.issue(kb, ks.lo + (t + 2) * kKT, ks.hi, lds + st * kTile);
-            if (!active) continue;
-            f32x4 sn[4][2];
-            if (t + 1 < n) scores(lds + (1 - st) * kTile, sn);
-            V8 pf[2][2];
+            if (MORE) lv.issue(vb, ks.lo + (t + 1) * BK, ks.hi, lds + (3 - st) * kStage);
+            if (t + 2 < n) lk.issue(kb, ks.lo + (t + 2) * BK, ks.hi, lds + st * kStage);
+            if (!active) return;
+            if (MORE) scores(lds + (1 - st) * kStage + kg * kTile, sn);
+            V8 pf[NT][kP];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int k2 = 0; k2 < kP; ++k2)
 #pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) {
+                for (int j = 0; j < NT; ++j) {
 #pragma unroll
                     for (int i = 2 * k2; i < 2 * k2 + 2; ++i)
 #pragma unroll
@@ -148,26 +166,83 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
                         }
                     pf[j][k2] = pack_frag<T>(s[2 * k2][j], s[2 * k2 + 1][j]);
                 }
-            const uint8_t* vt = lds + (2 + st) * kTile;
+            const uint8_t* vt = lds + (2 + st) * kStage + kg * kTile;
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2)
+            for (int k2 = 0; k2 < kP; ++k2)
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
                     const V8 f = tr_frag<T, D>(vt, fa.tr, k2, i);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) o[i][j] = AttnMma<T>::run(f, pf[j][k2], o[i][j]);
+                    for (int j = 0; j < NT; ++j) o[i][j] = AttnMma<T>::run(f, pf[j][k2], o[i][j]);
                 }
-            if (t + 1 < n) {
+            if (MORE) {
+                tops(sn, top);
+                const int left = mine - (t + 1) * BK;
+                if (left < KT) {
+                    mask(sn, left);
+                    tops(sn, top);
+                }
+                follow(top);
+            }
+        };
+        constexpr std::true_type more{};
+        constexpr std::false_type last{};
+        int t = 0;
+        for (; t + 2 < n; t += 2) {
+            tile(more, t, sa, sb);
+            tile(more, t + 1, sb, sa);
+        }
+        if (t + 1 < n) {
+            tile(more, t, sa, sb);
+            tile(last, t + 1, sb, sa);
+        } else {
+            tile(last, t, sa, sb);
+        }
+    }
+    if constexpr (KG > 1) {
+        // join of the groups: reference, sum and output of groups 1.. through LDS
+        constexpr int kFrags = D / 16 * NT;
+        static_assert((KG - 1) * NW * (kFrags * 16 + NT * 12) * 64 <= 4 * kStage, "the join fits the tiles' LDS");
+        f32x4* po = reinterpret_cast<f32x4*>(lds);
+        float* pm = reinterpret_cast<float*>(lds + (KG - 1) * NW * kFrags * 1024);
+        wait_lds_reads();
+        tile_barrier();
+        if (kg > 0) {
+            const int at = wave - NW;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[i][0] = sn[i][0], s[i][1] = sn[i][1];
-                if (t + 2 == n) mask(s, ks.hi - ks.lo - (t + 1) * kKT);
-                follow(s);
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) po[(at * kFrags + i * NT + j) * 64 + lane] = o[i][j];
+                float* m = pm + ((at * NT + j) * 64 + lane) * 3;
+                m[0] = mc[j];
+                m[1] = thr[j];
+                m[2] = l[j];
+            }
+        }
+        wait_lds_reads();
+        tile_barrier();
+        if (kg > 0) return;
+#pragma unroll
+        for (int g = 1; g < KG; ++g) {
+            const int at = (g - 1) * NW + qw;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const float* m = pm + ((at * NT + j) * 64 + lane) * 3;
+                const float m1 = m[0], t1 = m[1], l1 = m[2];
+                if (t1 == -INFINITY) continue;      // a group without keys
+                const float top = thr[j] == -INFINITY ? m1 : fmaxf(mc[j], m1);
+                const float w0 = thr[j] == -INFINITY ? 0.0f : exp2_f(mc[j] - top), w1 = exp2_f(m1 - top);
+                mc[j] = top;
+                thr[j] = t1;
+                l[j] = fmaf(l[j], w0, l1 * w1);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[i][j] = o[i][j] * w0 + po[(at * kFrags + i * NT + j) * 64 + lane] * w1;
             }
         }
     }
     if (!active) return;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NT; ++j) {
         l[j] += __shfl_xor(l[j], 16);
         l[j] += __shfl_xor(l[j], 32);
         const int row = q0 + 16 * j + r;
@@ -193,49 +268,117 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_kernel(AttnArgs a) {
     }
 }
 
-// Join of the splits: out = sum_s exp2(lse_s - lse) out_s. One DPP row of 16
-// lanes per (row, head), D / 16 elements a lane.
-template <typename T, int D>
+// Join of the splits: out = sum_s exp2(lse_s - lse) out_s. A wave takes STRANDS
+// splits at a time of 4 / STRANDS (row, head)s, 16 lanes each, D / 16 elements a
+// lane; WAVES waves share a (row, head)'s splits and meet in LDS.
+template <typename T, int D, int STRANDS, int WAVES>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    constexpr int E = D / 16;
-    const int64_t u = block_linear() * 16 + threadIdx.x / 16;
-    if (u >= a.q_rows * a.heads) return;
+    constexpr int E = D / 16, kUnits = 16 / (STRANDS * WAVES);
+    static_assert(STRANDS == 1 || STRANDS == 4, "lanes");
+    const int wave = threadIdx.x >> 6, lane = lane_id(), m = lane & 15, h = lane >> 4;
+    const int64_t total = a.q_rows * a.heads;
+    const int64_t u0 = block_linear() * kUnits + (STRANDS == 1 ? (WAVES == 1 ? wave * 4 + h : h) : (WAVES == 1 ? wave : 0));
+    const int64_t u = u0 < total ? u0 : total - 1;
+    const int first = STRANDS == 1 ? (WAVES == 1 ? 0 : wave) : (WAVES == 1 ? h : wave * 4 + h);
     const int64_t row = u / a.heads;
     const int head = (int)(u - row * a.heads);
-    const int m = threadIdx.x & 15;
-    if (a.qs.offsets != nullptr && (row < a.qs.offsets[0] || row >= a.qs.offsets[a.nbatch])) return;
-    float top = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.part_lse[((int64_t)s * a.heads + head) * a.q_rows + row]);
-    float acc[E] = {}, sum = 0.0f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float l = a.part_lse[((int64_t)s * a.heads + head) * a.q_rows + row];
-        const float w = l == -INFINITY ? 0.0f : exp2_f(l - top);
+    const float* pl = a.part_lse + head * a.q_rows + row;
+    const float* po = a.part + (row * a.heads + head) * D + m * E;
+    const int64_t ls = a.heads * a.q_rows, os = ls * D;
+    float top = -INFINITY, sum = 0.0f, acc[E] = {};
+#pragma unroll 4
+    for (int s = first; s < a.nsplit; s += STRANDS * WAVES) {
+        const float l = pl[s * ls];
         float v[E];
-        load_params<E>(a.part + (((int64_t)s * a.q_rows + row) * a.heads + head) * D + m * E, v);
+        load_params<E>(po + s * os, v);
+        const float t = fmaxf(top, l);
+        const float w0 = top == -INFINITY ? 0.0f : exp2_f(top - t), w1 = l == -INFINITY ? 0.0f : exp2_f(l - t);
+        top = t;
+        sum = fmaf(sum, w0, w1);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[e], acc[e]);
-        sum += w;
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + v[e] * w1;
     }
+    const auto join = [&](float t1, float s1, const float (&v)[E]) {
+        const float t = fmaxf(top, t1);
+        const float w0 = top == -INFINITY ? 0.0f : exp2_f(top - t), w1 = t1 == -INFINITY ? 0.0f : exp2_f(t1 - t);
+        top = t;
+        sum = sum * w0 + s1 * w1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + v[e] * w1;
+    };
+    if constexpr (STRANDS == 4) {
+#pragma unroll
+        for (int x = 16; x < 64; x <<= 1) {
+            const float t1 = __shfl_xor(top, x), s1 = __shfl_xor(sum, x);
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = __shfl_xor(acc[e], x);
+            join(t1, s1, v);
+        }
+    }
+    if constexpr (WAVES > 1) {
+        __shared__ float lt[WAVES][16], lm[WAVES][16], lo[WAVES][16][E];
+        if (h == 0) {
+            lt[wave][m] = top;
+            lm[wave][m] = sum;
+#pragma unroll
+            for (int e = 0; e < E; ++e) lo[wave][m][e] = acc[e];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+        for (int w = 1; w < WAVES; ++w) {
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = lo[w][m][e];
+            join(lt[w][m], lm[w][m], v);
+        }
+    }
+    if (u0 >= total || (STRANDS == 4 && h > 0)) return;
+    if (a.qs.offsets != nullptr && (row < a.qs.offsets[0] || row >= a.qs.offsets[a.nbatch])) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= inv;
-    store_elems<T, E>(static_cast<T*>(a.out) + (int64_t)row * a.o_row + head * a.o_head + m * E, acc);
+    store_elems<T, E>(static_cast<T*>(a.out) + row * a.o_row + head * a.o_head + m * E, acc);
     if (a.lse != nullptr && m == 0)
         a.lse[head * a.q_rows + row] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-constexpr int kWaves = 8;
+// The kernel's forms: waves, 16-query tiles a wave, keys of a wave's tile, key
+// groups.
+struct Large { static constexpr int nw = 8, nt = 2, kt = 64; template <int D> static constexpr int kg = 1; };
+struct Medium { static constexpr int nw = 4, nt = 2, kt = 64; template <int D> static constexpr int kg = 1; };
+struct Small { static constexpr int nw = 4, nt = 1, kt = 64; template <int D> static constexpr int kg = 1; };
+struct Few { static constexpr int nw = 1, nt = 1, kt = 32; template <int D> static constexpr int kg = D == 64 ? 8 : 4; };
+enum Form { kLarge, kMedium, kSmall, kFew };
+
+Form form_of(const AttnArgs& a) {
+    const int64_t rows = (a.q_rows + a.nbatch - 1) / a.nbatch, cu = device_cu_count();
+    if (rows <= 16) return kFew;
+    const int64_t per = (int64_t)a.nbatch * a.heads;
+    if ((rows + 127) / 128 * per * 2 < cu * 3) return kSmall;
+    return (rows + 255) / 256 * per < cu * 3 ? kMedium : kLarge;
+}
+
+template <typename T, int D, typename F, bool SPLIT>
+void launch_form(AttnArgs& a, hipStream_t s) {
+    a.q_tiles = (int32_t)tile_count(a.qs, a.nbatch, F::nw * F::nt * 16);
+    a.nblocks = a.q_tiles * a.nsplit * a.heads;
+    constexpr int kg = F::template kg<D>;
+    hipLaunchKernelGGL((attn_kernel<T, D, F::nw, F::nt, F::kt, kg, SPLIT>), grid_1d(a.nblocks), dim3(F::nw * kg * 64), 0, s, a);
+}
 
 template <typename T, int D>
 hipError_t launch_d(AttnArgs a, hipStream_t s) {
-    a.q_tiles = (int32_t)tile_count(a.qs, a.nbatch, kWaves * 32);
-    a.nblocks = a.q_tiles * a.nsplit * a.heads;
+    switch (form_of(a)) {
+        case kLarge: launch_form<T, D, Large, false>(a, s); break;
+        case kMedium: launch_form<T, D, Medium, false>(a, s); break;
+        case kSmall: a.nsplit > 1 ? launch_form<T, D, Small, true>(a, s) : launch_form<T, D, Small, false>(a, s); break;
+        default: a.nsplit > 1 ? launch_form<T, D, Few, true>(a, s) : launch_form<T, D, Few, false>(a, s);
+    }
     if (a.nsplit > 1) {
-        hipLaunchKernelGGL((attn_kernel<T, D, kWaves, true>), grid_1d(a.nblocks), dim3(kWaves * 64), 0, s, a);
-        const int64_t nb = (a.q_rows * a.heads + 15) / 16;
-        hipLaunchKernelGGL((attn_join_kernel<T, D>), grid_1d(nb), dim3(256), 0, s, a);
-    } else {
-        hipLaunchKernelGGL((attn_kernel<T, D, kWaves, false>), grid_1d(a.nblocks), dim3(kWaves * 64), 0, s, a);
+        const int64_t units = a.q_rows * a.heads;
+        if (a.nsplit > 8) hipLaunchKernelGGL((attn_join_kernel<T, D, 4, 4>), grid_1d(units), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((attn_join_kernel<T, D, 1, 1>), grid_1d((units + 15) / 16), dim3(256), 0, s, a);
     }
     return hipGetLastError();
 }
@@ -243,11 +386,13 @@ hipError_t launch_d(AttnArgs a, hipStream_t s) {
 }  // namespace
 
 int attn_splits(const AttnArgs& a) {
-    const int64_t tiles = tile_count(a.qs, a.nbatch, kWaves * 32) * a.heads;
-    const int64_t cu = device_cu_count();
-    const int64_t keys = a.k_rows / a.nbatch;
-    int64_t n = cu / (tiles > 0 ? tiles : 1);
-    if (n > keys / 128) n = keys / 128;
+    const int64_t rows = (a.q_rows + a.nbatch - 1) / a.nbatch, keys = a.k_rows / a.nbatch;
+    const Form f = form_of(a);
+    if (f != kSmall && f != kFew) return 1;
+    const int64_t tiles = (rows + (f == kFew ? 15 : 63)) / (f == kFew ? 16 : 64) * a.nbatch * a.heads;
+    int64_t n = device_cu_count() / (tiles > 0 ? tiles : 1);
+    const int64_t least = f == kFew ? 1024 : 128;
+    if (n > keys / least) n = keys / least;
     if (n > 64) n = 64;
     return n < 1 ? 1 : (int)n;
 }

@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
     int b;
     if (u < qb) {
         const int head = u / a.prep_q_tiles;
-        const Rows s = tile_rows<kPrepRows>(f.qs, f.nbatch, u - head * a.prep_q_tiles, b);
+        const Rows s = tile_rows<kPrepRows>(f.qs, f.nbatch, u - head * a.prep_q_tiles, lane_id(), b);
 #pragma unroll
         for (int i = 0; i < kPrepRows / 16; ++i) {
             const int64_t row = s.lo + i * 16 + rr;
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
     } else {
         const int w = u - qb;
         const int head = w / a.prep_k_tiles;
-        Rows s = tile_rows<kPrepRows>(f.ks, f.nbatch, w - head * a.prep_k_tiles, b);
+        Rows s = tile_rows<kPrepRows>(f.ks, f.nbatch, w - head * a.prep_k_tiles, lane_id(), b);
         const int end = segment_keys(f, b).hi;
         s.hi = end < s.hi ? end : s.hi;
 #pragma unroll
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a
     const int rem = u - kvh * per_head;
     const int split = SPLIT ? rem / a.k_tiles : 0;
     int b;
-    const Rows ks = tile_rows<BK>(f.ks, f.nbatch, rem - split * a.k_tiles, b);
+    const Rows ks = tile_rows<BK>(f.ks, f.nbatch, rem - split * a.k_tiles, lane_id(), b);
     if (ks.lo >= ks.hi) return;
     const Rows qs = segment_rows(f.qs, b);
     // keys from k_end on do not count: their gradients are zero
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dq_kernel(AttnBwdArgs a)
     const int rem = u - head * per_head;
     const int split = SPLIT ? rem / f.q_tiles : 0;
     int b;
-    const Rows qs = tile_rows<BQ>(f.qs, f.nbatch, rem - split * f.q_tiles, b);
+    const Rows qs = tile_rows<BQ>(f.qs, f.nbatch, rem - split * f.q_tiles, lane_id(), b);
     if (qs.lo >= qs.hi) return;
     Rows ks = segment_keys(f, b);
     const int keys = ks.hi - ks.lo;
