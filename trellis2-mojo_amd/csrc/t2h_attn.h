@@ -45,8 +45,9 @@ struct AttnBwdArgs {
     void* dv;
     int64_t do_row, do_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
     int32_t kv_heads;
-    // set by attn_bwd_plan: parts, and the workspace's pieces
+    // set by attn_bwd_plan: forms, parts, and the workspace's pieces
     int32_t kv_split, q_split;
+    bool kv_small, q_small;
     float* delta;            // [heads, q_rows]
     float* lse2;             // [heads, q_rows] log2, less the rounding shift of P
     float* g_most;           // [heads, prep_q_tiles] f16: largest squared row length of dout in each tile

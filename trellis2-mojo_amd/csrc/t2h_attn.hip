@@ -345,18 +345,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 // The kernel's forms: waves, 16-query tiles a wave, keys of a wave's tile, key
 // groups.
-struct Large { static constexpr int nw = 8, nt = 2, kt = 64; template <int D> static constexpr int kg = 1; };
-struct Medium { static constexpr int nw = 4, nt = 2, kt = 64; template <int D> static constexpr int kg = 1; };
+struct Large { static constexpr int nw = 4, nt = 2, kt = 64; template <int D> static constexpr int kg = 1; };
 struct Small { static constexpr int nw = 4, nt = 1, kt = 64; template <int D> static constexpr int kg = 1; };
 struct Few { static constexpr int nw = 1, nt = 1, kt = 32; template <int D> static constexpr int kg = D == 64 ? 8 : 4; };
-enum Form { kLarge, kMedium, kSmall, kFew };
+enum Form { kLarge, kSmall, kFew };
 
 Form form_of(const AttnArgs& a) {
     const int64_t rows = (a.q_rows + a.nbatch - 1) / a.nbatch, cu = device_cu_count();
     if (rows <= 16) return kFew;
     const int64_t per = (int64_t)a.nbatch * a.heads;
-    if ((rows + 127) / 128 * per * 2 < cu * 3) return kSmall;
-    return (rows + 255) / 256 * per < cu * 3 ? kMedium : kLarge;
+    return (rows + 127) / 128 * per * 2 < cu * 3 ? kSmall : kLarge;
 }
 
 template <typename T, int D, typename F, bool SPLIT>
@@ -371,7 +369,6 @@ template <typename T, int D>
 hipError_t launch_d(AttnArgs a, hipStream_t s) {
     switch (form_of(a)) {
         case kLarge: launch_form<T, D, Large, false>(a, s); break;
-        case kMedium: launch_form<T, D, Medium, false>(a, s); break;
         case kSmall: a.nsplit > 1 ? launch_form<T, D, Small, true>(a, s) : launch_form<T, D, Small, false>(a, s); break;
         default: a.nsplit > 1 ? launch_form<T, D, Few, true>(a, s) : launch_form<T, D, Few, false>(a, s);
     }

@@ -5,11 +5,10 @@
 //   dP_ij = dout_i.v_j                     dS_ij = P_ij (dP_ij - delta_i)
 //   dv_j = sum_i P_ij dout_i    dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i
 //
-// Three launches: delta (and, for f16, the largest row lengths); dk and dv with
-// the keys kept in registers and the queries streaming; dq with the queries
-// kept and the keys streaming. The last two compute P and dP twice, seven
-// products in place of five, and need no atomic sums, whose order would change
-// the result from run to run.
+// Two launches: dq (and delta) with the queries kept in registers and the keys
+// streaming; dk and dv with the keys kept and the queries streaming. They
+// compute P and dP twice, seven products in place of five, and need no atomic
+// sums, whose order would change the result from run to run.
 //
 // f16: P is rounded as 2^14 P (P is near 1 / keys, below f16's smallest normal
 // number from 16,384 keys on), and dS as 2^e dS, e a power of two from the bound
@@ -42,11 +41,11 @@ __device__ __forceinline__ float shift_ds(float g2, float v2) {
     return (float)e;
 }
 
-// ---- delta and row lengths ----------------------------------------------------
-// A block takes up to kPrepRows rows of one segment and one head of dout and out
-// (or, f16, of v; only keys that count), 16 lanes a row.
+// ---- row lengths (f16) ----------------------------------------------------------
+// A block takes up to kPrepRows rows of one segment and one head of dout or of v
+// (only keys that count), 16 lanes a row.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
+__global__ __launch_bounds__(256) void attn_lengths_kernel(AttnBwdArgs a) {
     constexpr int E = D / 16;
     const AttnArgs& f = a.f;
     const int64_t p = block_linear();
@@ -54,68 +53,233 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
     const int u = (int)p;
     const int m = threadIdx.x & 15, rr = threadIdx.x >> 4;
     const int qb = a.prep_q_tiles * f.heads;
-    __shared__ float top[16];
-    float most = 0.0f;
+    const bool q = u < qb;
+    const int per = q ? a.prep_q_tiles : a.prep_k_tiles, w = q ? u : u - qb;
+    const int head = w / per;
     int b;
-    if (u < qb) {
-        const int head = u / a.prep_q_tiles;
-        const Rows s = tile_rows<kPrepRows>(f.qs, f.nbatch, u - head * a.prep_q_tiles, lane_id(), b);
-#pragma unroll
-        for (int i = 0; i < kPrepRows / 16; ++i) {
-            const int64_t row = s.lo + i * 16 + rr;
-            if (row >= s.hi) break;
-            float g[E], o[E];
-            load_elems<T, E>(static_cast<const T*>(a.dout) + row * a.do_row + head * a.do_head + m * E, g);
-            load_elems<T, E>(static_cast<const T*>(f.out) + row * f.o_row + head * f.o_head + m * E, o);
-            float d = 0.0f, g2 = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                d = fmaf(g[e], o[e], d);
-                g2 = fmaf(g[e], g[e], g2);
-            }
-            d = row16_sum(d);
-            if (HalfRange<T>::value) most = fmaxf(most, row16_sum(g2));
-            if (m == 0) {
-                const int64_t at = head * f.q_rows + row;
-                const float lse = f.lse[at];
-                a.delta[at] = d;
-                a.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e - (HalfRange<T>::value ? kShiftP : 0.0f);
-            }
-        }
-    } else {
-        const int w = u - qb;
-        const int head = w / a.prep_k_tiles;
-        Rows s = tile_rows<kPrepRows>(f.ks, f.nbatch, w - head * a.prep_k_tiles, lane_id(), b);
+    Rows s = tile_rows<kPrepRows>(q ? f.qs : f.ks, f.nbatch, w - head * per, lane_id(), b);
+    if (!q) {
         const int end = segment_keys(f, b).hi;
         s.hi = end < s.hi ? end : s.hi;
+    }
+    const T* x = q ? static_cast<const T*>(a.dout) + head * a.do_head : static_cast<const T*>(f.v) + head * f.v_head;
+    const int64_t stride = q ? a.do_row : f.v_row;
+    __shared__ float top[16];
+    float most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kPrepRows / 16; ++i) {
-            const int64_t row = s.lo + i * 16 + rr;
-            if (row >= s.hi) break;
-            float v[E];
-            load_elems<T, E>(static_cast<const T*>(f.v) + row * f.v_row + head * f.v_head + m * E, v);
-            most = fmaxf(most, row16_sum(sum_sq_all<E>(v)));
+    for (int i = 0; i < kPrepRows / 16; ++i) {
+        const int row = s.lo + i * 16 + rr;
+        if (row >= s.hi) break;
+        float v[E];
+        load_elems<T, E>(x + row * stride + m * E, v);
+        most = fmaxf(most, row16_sum(sum_sq_all<E>(v)));
+    }
+    if (m == 0) top[rr] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, top[i]);
+        (q ? a.g_most : a.v_most)[w] = most;
+    }
+}
+
+// ---- dq -------------------------------------------------------------------------
+constexpr int kKT = 64;   // keys per tile
+
+template <typename T, int D, int NW, int NT, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnBwdArgs a) {
+    using V8 = typename AttnMma<T>::v8;
+    constexpr int BQ = NW * NT * 16;
+    constexpr int kTile = kKT * D * 2;
+    constexpr bool kF16 = HalfRange<T>::value;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];   // k, k, v, v
+    const AttnArgs& f = a.f;
+    const int64_t p = block_linear();
+    if (p >= a.q_blocks) return;
+    const int u = xcd_order((int)p, a.q_blocks);
+    const int per_head = f.q_tiles * a.q_split;
+    const int head = u / per_head;
+    const int rem = u - head * per_head;
+    const int split = SPLIT ? rem / f.q_tiles : 0;
+    int b;
+    const Rows qs = tile_rows<BQ>(f.qs, f.nbatch, rem - split * f.q_tiles, lane_id(), b);
+    if (qs.lo >= qs.hi) return;
+    Rows ks = segment_keys(f, b);
+    const int keys = ks.hi - ks.lo;
+    if constexpr (SPLIT) {
+        const int tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
+        const int t0 = (int)((int64_t)tiles * split / a.q_split), t1 = (int)((int64_t)tiles * (split + 1) / a.q_split);
+        if (t1 < tiles) ks.hi = ks.lo + t1 * kKT;
+        ks.lo += t0 * kKT;
+    }
+    const int n = ks.hi > ks.lo ? (ks.hi - ks.lo + kKT - 1) / kKT : 0;
+
+    const int lane = lane_id(), r = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int q0 = qs.lo + wave * (NT * 16);
+    const bool active = q0 < qs.hi;
+    const int kvh = head / f.group;
+    const uint8_t* kb = static_cast<const uint8_t*>(f.k) + kvh * f.k_head * 2;
+    const uint8_t* vb = static_cast<const uint8_t*>(f.v) + kvh * f.v_head * 2;
+    TileLoad<D, kKT, NW> lk, lv;
+    lk.init(wave, lane, f.k_row);
+    lv.init(wave, lane, f.v_row);
+    const FragAddr<D> fa(lane);
+    const float c = f.scale * kLog2e;
+
+    V8 q[NT][D / 32], g[NT][D / 32];
+    f32x4 dq[D / 16][NT];
+    float l2[NT], de[NT], z[NT], w[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) dq[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        l2[j] = INFINITY;
+        de[j] = 0.0f;
+        z[j] = 1.0f;
+        w[j] = f.scale;
+    }
+    if (n > 0) {
+        lk.issue(kb, ks.lo, ks.hi, lds);
+        lv.issue(vb, ks.lo, ks.hi, lds + 2 * kTile);
+    }
+    if (active && (n > 0 || split == 0)) {
+        float v2 = 0.0f;
+        if constexpr (kF16) v2 = largest(a.v_most + kvh * a.prep_k_tiles + first_tile<kPrepRows>(f.ks, b), keys, lane);
+        const uint8_t* qb = static_cast<const uint8_t*>(f.q) + (head * f.q_head + (int64_t)q0 * f.q_row) * 2;
+        const uint8_t* gb = static_cast<const uint8_t*>(a.dout) + (head * a.do_head + (int64_t)q0 * a.do_row) * 2;
+        const uint8_t* ob = static_cast<const uint8_t*>(f.out) + (head * f.o_head + (int64_t)q0 * f.o_row) * 2;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            V8 o[D / 32];
+            load_own<T, D>(q[j], qb + 16 * j * f.q_row * 2, qs.hi - q0 - 16 * j, (uint32_t)f.q_row * 2, lane);
+            load_own<T, D>(g[j], gb + 16 * j * a.do_row * 2, qs.hi - q0 - 16 * j, (uint32_t)a.do_row * 2, lane);
+            load_own<T, D>(o, ob + 16 * j * f.o_row * 2, qs.hi - q0 - 16 * j, (uint32_t)f.o_row * 2, lane);
+            const int row = q0 + 16 * j + r;
+            const float lse = row < qs.hi ? f.lse[head * f.q_rows + row] : -INFINITY;
+            float g2 = 0.0f;
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = (float)g[j][t][e];
+                    de[j] = fmaf(x, (float)o[t][e], de[j]);
+                    if (kF16) g2 = fmaf(x, x, g2);
+                }
+            de[j] += __shfl_xor(de[j], 16);
+            de[j] += __shfl_xor(de[j], 32);
+            // a row without keys: P = 0
+            l2[j] = lse == -INFINITY ? INFINITY : lse * kLog2e - (kF16 ? kShiftP : 0.0f);
+            if (split == 0 && h == 0 && row < qs.hi) {      // for dk and dv
+                a.delta[head * f.q_rows + row] = de[j];
+                a.lse2[head * f.q_rows + row] = l2[j];
+            }
+            if constexpr (kF16) {
+                g2 += __shfl_xor(g2, 16);
+                g2 += __shfl_xor(g2, 32);
+                const float e = shift_ds(g2, v2);
+                z[j] = exp2_f(e - kShiftP);
+                de[j] *= z[j];
+                w[j] = f.scale * exp2_f(-e);
+            }
         }
     }
-    if constexpr (HalfRange<T>::value) {
-        if (m == 0) top[rr] = most;
-        __syncthreads();
-        if (threadIdx.x == 0) {
+    if (n > 0) {
+        for (int t = 0; t < n; ++t) {
+            const int st = t & 1;
+            wait_loads<0>();
+            wait_lds_reads();
+            tile_barrier();
+            if (t + 1 < n) {
+                lk.issue(kb, ks.lo + (t + 1) * kKT, ks.hi, lds + (1 - st) * kTile);
+                lv.issue(vb, ks.lo + (t + 1) * kKT, ks.hi, lds + (3 - st) * kTile);
+            }
+            if (!active) continue;
+            const int left = ks.hi - ks.lo - t * kKT;
+            const uint8_t* kt = lds + st * kTile;
+            const uint8_t* vt = lds + (2 + st) * kTile;
 #pragma unroll
-            for (int i = 1; i < 16; ++i) most = fmaxf(most, top[i]);
-            (u < qb ? a.g_most : a.v_most)[u < qb ? u : u - qb] = most;
+            for (int s2 = 0; s2 < kKT / 32; ++s2) {
+                f32x4 s[2][NT], d[2][NT];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) s[i][j] = d[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const V8 y = row_frag<T, D>(kt, fa.row, 2 * s2 + i, x);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) s[i][j] = AttnMma<T>::run(y, q[j][x], s[i][j]);
+                    }
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const V8 y = row_frag<T, D>(vt, fa.row, 2 * s2 + i, x);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) d[i][j] = AttnMma<T>::run(y, g[j][x], d[i][j]);
+                    }
+                // keys past the last: their score 0 may be far above lse, and P with it beyond any number
+                if (left < kKT) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (32 * s2 + 16 * i + 4 * h + e >= left) {
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) s[i][j][e] = -INFINITY;
+                            }
+                }
+                V8 df[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float pr = exp2_f(fmaf(s[i][j][e], c, -l2[j]));
+                            d[i][j][e] = pr * (kF16 ? fmaf(d[i][j][e], z[j], -de[j]) : d[i][j][e] - de[j]);
+                        }
+                    df[j] = pack_frag<T>(d[0][j], d[1][j]);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const V8 x = tr_frag<T, D>(kt, fa.tr, s2, i);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) dq[i][j] = AttnMma<T>::run(x, df[j], dq[i][j]);
+                }
+            }
+        }
+    }
+    if (!active) return;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int row = q0 + 16 * j + r;
+        if (row >= qs.hi) continue;
+        if constexpr (SPLIT) {
+            float* po = a.part + (((int64_t)split * f.q_rows + row) * f.heads + head) * D + 4 * h;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(po + 16 * i) = dq[i][j] * w[j];
+        } else {
+            T* po = static_cast<T*>(a.dq) + (int64_t)row * a.dq_row + head * a.dq_head + 4 * h;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                typename AttnMma<T>::v4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (T)(dq[i][j][e] * w[j]);
+                *reinterpret_cast<typename AttnMma<T>::v4*>(po + 16 * i) = x;
+            }
         }
     }
 }
 
 // ---- dk, dv ---------------------------------------------------------------------
-#ifndef T2H_DKV_UNROLL
-#define T2H_DKV_UNROLL 1
-#endif
 constexpr int kQT = 64;   // queries per tile
 
 template <typename T, int D, int NW, int NT, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
     using V8 = typename AttnMma<T>::v8;
     constexpr int BK = NW * NT * 16;
     constexpr int kTile = kQT * D * 2;
@@ -212,7 +376,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a
             const uint8_t* gt = lds + (2 + st) * kTile;
             const float* ls = reinterpret_cast<const float*>(lds + 4 * kTile) + st * kQT;
             const float* de = ls + 2 * kQT;
-#pragma unroll T2H_DKV_UNROLL
+#pragma unroll 1
             for (int s2 = 0; s2 < kQT / 32; ++s2) {
                 f32x4 s[2][NT], d[2][NT];
 #pragma unroll
@@ -302,185 +466,6 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_dkv_kernel(AttnBwdArgs a
     }
 }
 
-// ---- dq -------------------------------------------------------------------------
-constexpr int kKT = 64;   // keys per tile
-
-template <typename T, int D, int NW, int NT, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, NW / 4) void attn_dq_kernel(AttnBwdArgs a) {
-    using V8 = typename AttnMma<T>::v8;
-    constexpr int BQ = NW * NT * 16;
-    constexpr int kTile = kKT * D * 2;
-    constexpr bool kF16 = HalfRange<T>::value;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];   // k, k, v, v
-    const AttnArgs& f = a.f;
-    const int64_t p = block_linear();
-    if (p >= a.q_blocks) return;
-    const int u = xcd_order((int)p, a.q_blocks);
-    const int per_head = f.q_tiles * a.q_split;
-    const int head = u / per_head;
-    const int rem = u - head * per_head;
-    const int split = SPLIT ? rem / f.q_tiles : 0;
-    int b;
-    const Rows qs = tile_rows<BQ>(f.qs, f.nbatch, rem - split * f.q_tiles, lane_id(), b);
-    if (qs.lo >= qs.hi) return;
-    Rows ks = segment_keys(f, b);
-    const int keys = ks.hi - ks.lo;
-    if constexpr (SPLIT) {
-        const int tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
-        const int t0 = (int)((int64_t)tiles * split / a.q_split), t1 = (int)((int64_t)tiles * (split + 1) / a.q_split);
-        if (t1 < tiles) ks.hi = ks.lo + t1 * kKT;
-        ks.lo += t0 * kKT;
-    }
-    const int n = ks.hi > ks.lo ? (ks.hi - ks.lo + kKT - 1) / kKT : 0;
-
-    const int lane = lane_id(), r = lane & 15, h = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int q0 = qs.lo + wave * (NT * 16);
-    const bool active = q0 < qs.hi;
-    const int kvh = head / f.group;
-    const uint8_t* kb = static_cast<const uint8_t*>(f.k) + kvh * f.k_head * 2;
-    const uint8_t* vb = static_cast<const uint8_t*>(f.v) + kvh * f.v_head * 2;
-    TileLoad<D, kKT, NW> lk, lv;
-    lk.init(wave, lane, f.k_row);
-    lv.init(wave, lane, f.v_row);
-    const FragAddr<D> fa(lane);
-    const float c = f.scale * kLog2e;
-
-    V8 q[NT][D / 32], g[NT][D / 32];
-    f32x4 dq[D / 16][NT];
-    float l2[NT], de[NT], z[NT], w[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) dq[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        l2[j] = INFINITY;
-        de[j] = 0.0f;
-        z[j] = 1.0f;
-        w[j] = f.scale;
-    }
-    if (n > 0) {
-        lk.issue(kb, ks.lo, ks.hi, lds);
-        lv.issue(vb, ks.lo, ks.hi, lds + 2 * kTile);
-        if (active) {
-            float v2 = 0.0f;
-            if constexpr (kF16)
-                v2 = largest(a.v_most + kvh * a.prep_k_tiles + first_tile<kPrepRows>(f.ks, b), keys, lane);
-            const uint8_t* qb = static_cast<const uint8_t*>(f.q) + (head * f.q_head + (int64_t)q0 * f.q_row) * 2;
-            const uint8_t* gb = static_cast<const uint8_t*>(a.dout) + (head * a.do_head + (int64_t)q0 * a.do_row) * 2;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                load_own<T, D>(q[j], qb + 16 * j * f.q_row * 2, qs.hi - q0 - 16 * j, (uint32_t)f.q_row * 2, lane);
-                load_own<T, D>(g[j], gb + 16 * j * a.do_row * 2, qs.hi - q0 - 16 * j, (uint32_t)a.do_row * 2, lane);
-                const int row = q0 + 16 * j + r;
-                if (row < qs.hi) {
-                    l2[j] = a.lse2[head * f.q_rows + row];
-                    de[j] = a.delta[head * f.q_rows + row];
-                }
-                if constexpr (kF16) {
-                    float g2 = 0.0f;
-#pragma unroll
-                    for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) g2 = fmaf((float)g[j][t][e], (float)g[j][t][e], g2);
-                    g2 += __shfl_xor(g2, 16);
-                    g2 += __shfl_xor(g2, 32);
-                    const float e = shift_ds(g2, v2);
-                    z[j] = exp2_f(e - kShiftP);
-                    de[j] *= z[j];
-                    w[j] = f.scale * exp2_f(-e);
-                }
-            }
-        }
-        for (int t = 0; t < n; ++t) {
-            const int st = t & 1;
-            wait_loads<0>();
-            wait_lds_reads();
-            tile_barrier();
-            if (t + 1 < n) {
-                lk.issue(kb, ks.lo + (t + 1) * kKT, ks.hi, lds + (1 - st) * kTile);
-                lv.issue(vb, ks.lo + (t + 1) * kKT, ks.hi, lds + (3 - st) * kTile);
-            }
-            if (!active) continue;
-            const int left = ks.hi - ks.lo - t * kKT;
-            const uint8_t* kt = lds + st * kTile;
-            const uint8_t* vt = lds + (2 + st) * kTile;
-#pragma unroll
-            for (int s2 = 0; s2 < kKT / 32; ++s2) {
-                f32x4 s[2][NT], d[2][NT];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) s[i][j] = d[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const V8 y = row_frag<T, D>(kt, fa.row, 2 * s2 + i, x);
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) s[i][j] = AttnMma<T>::run(y, q[j][x], s[i][j]);
-                    }
-#pragma unroll
-                for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const V8 y = row_frag<T, D>(vt, fa.row, 2 * s2 + i, x);
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) d[i][j] = AttnMma<T>::run(y, g[j][x], d[i][j]);
-                    }
-                // keys past the last: their score 0 may be far above lse, and P with it beyond any number
-                if (left < kKT) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (32 * s2 + 16 * i + 4 * h + e >= left) {
-#pragma unroll
-                                for (int j = 0; j < NT; ++j) s[i][j][e] = -INFINITY;
-                            }
-                }
-                V8 df[NT];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float pr = exp2_f(fmaf(s[i][j][e], c, -l2[j]));
-                            d[i][j][e] = pr * (kF16 ? fmaf(d[i][j][e], z[j], -de[j]) : d[i][j][e] - de[j]);
-                        }
-                    df[j] = pack_frag<T>(d[0][j], d[1][j]);
-                }
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const V8 x = tr_frag<T, D>(kt, fa.tr, s2, i);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) dq[i][j] = AttnMma<T>::run(x, df[j], dq[i][j]);
-                }
-            }
-        }
-    }
-    if (!active) return;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int row = q0 + 16 * j + r;
-        if (row >= qs.hi) continue;
-        if constexpr (SPLIT) {
-            float* po = a.part + (((int64_t)split * f.q_rows + row) * f.heads + head) * D + 4 * h;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(po + 16 * i) = dq[i][j] * w[j];
-        } else {
-            T* po = static_cast<T*>(a.dq) + (int64_t)row * a.dq_row + head * a.dq_head + 4 * h;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                typename AttnMma<T>::v4 x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = (T)(dq[i][j][e] * w[j]);
-                *reinterpret_cast<typename AttnMma<T>::v4*>(po + 16 * i) = x;
-            }
-        }
-    }
-}
-
 // Sum of the parts [nsplit, rows, heads, D] in order; blockIdx.z: part set
 // (dk, dv) and output.
 struct SumArgs {
@@ -510,73 +495,114 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(SumArgs a) {
     store_elems<T, E>(static_cast<T*>(a.out[w]) + row * a.row_stride[w] + head * a.head_stride[w] + m * E, acc);
 }
 
-constexpr int kDqWaves = 8, kDqTiles = 2;
-#ifndef T2H_DKV_WAVES
-#define T2H_DKV_WAVES 8
-#define T2H_DKV_TILES 2
-#endif
-constexpr int kDkvWaves = T2H_DKV_WAVES, kDkvTiles = T2H_DKV_TILES;
-constexpr int kBQ = kDqWaves * kDqTiles * 16, kBK = kDkvWaves * kDkvTiles * 16;
+// The kernels' forms: waves and 16-token tiles a wave. Four waves, two blocks a
+// CU.
+struct Large { static constexpr int nw = 4, nt = 2; };
+struct Small { static constexpr int nw = 4, nt = 1; };
+constexpr int kRowsLarge = 128, kRowsSmall = 64;   // tokens a block keeps
+constexpr int kSplitRows = 1024;                   // streaming tokens that a part of the large form has at least
+
+// How one side's blocks take their work: the large form, its streaming side in as
+// many parts as the GPU's two blocks a CU take at once (39,804 queries of 1,029
+// keys, k_lens: dk, dv in 1 part and the rest of the pass 1,156 us, 2: 824, 3: 700, 4: 821;
+// 8,192 queries, all keys: 3 parts 174 us, 4: 141, 5: 185); where the parts would
+// be too short for 1.5 blocks a CU, the small form. padded: of the blocks' own
+// tokens only some count, three in four say.
+struct Plan { bool small; int split; };
+Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads, bool padded) {
+    const int64_t cu = device_cu_count(), per = (int64_t)nbatch * heads;
+    const int64_t large = ((int64_t)kept.share + kRowsLarge - 1) / kRowsLarge * per;
+    const int64_t small = ((int64_t)kept.share + kRowsSmall - 1) / kRowsSmall * per;
+    const int64_t most = stream / kSplitRows > 1 ? stream / kSplitRows : 1;
+    Plan p{};
+    p.small = large * most * 2 < 3 * cu;
+    int64_t n = 1;
+    if (p.small) {
+        n = cu / (small > 0 ? small : 1);
+        if (n > stream / 128) n = stream / 128;
+    } else if (large * 2 < 3 * cu) {
+        n = 2 * cu * (padded ? 4 : 3) / (large * 3);
+        if (n > most) n = most;
+    }
+    p.split = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    return p;
+}
+
+void launch_sums(const SumArgs& m, int sets, int32_t dtype, int32_t head_dim, hipStream_t s) {
+    dim3 grid = grid_1d((m.rows * m.heads + 15) / 16);
+    grid.z = sets;
+    if (dtype == T2H_F16) {
+        if (head_dim == 128) hipLaunchKernelGGL((attn_sum_kernel<_Float16, 128>), grid, dim3(256), 0, s, m);
+        else hipLaunchKernelGGL((attn_sum_kernel<_Float16, 64>), grid, dim3(256), 0, s, m);
+    } else {
+        if (head_dim == 128) hipLaunchKernelGGL((attn_sum_kernel<__bf16, 128>), grid, dim3(256), 0, s, m);
+        else hipLaunchKernelGGL((attn_sum_kernel<__bf16, 64>), grid, dim3(256), 0, s, m);
+    }
+}
+
+template <typename T, int D, typename F>
+void launch_dq(AttnBwdArgs& a, hipStream_t s) {
+    AttnArgs& f = a.f;
+    f.q_tiles = (int32_t)tile_count(f.qs, f.nbatch, F::nw * F::nt * 16);
+    a.q_blocks = f.q_tiles * a.q_split * f.heads;
+    if (a.q_blocks == 0) return;
+    if (a.q_split == 1) {
+        hipLaunchKernelGGL((attn_dq_kernel<T, D, F::nw, F::nt, false>), grid_1d(a.q_blocks), dim3(F::nw * 64), 0, s, a);
+        return;
+    }
+    hipLaunchKernelGGL((attn_dq_kernel<T, D, F::nw, F::nt, true>), grid_1d(a.q_blocks), dim3(F::nw * 64), 0, s, a);
+    SumArgs m{};
+    m.part[0] = a.part;
+    m.out[0] = a.dq;
+    m.row_stride[0] = a.dq_row;
+    m.head_stride[0] = a.dq_head;
+    m.offsets = f.qs.offsets;
+    m.rows = f.q_rows;
+    m.heads = f.heads;
+    m.nsplit = a.q_split;
+    m.nbatch = f.nbatch;
+    launch_sums(m, 1, f.dtype, D, s);
+}
+
+template <typename T, int D, typename F>
+void launch_dkv(AttnBwdArgs& a, hipStream_t s) {
+    const AttnArgs& f = a.f;
+    a.k_tiles = (int32_t)tile_count(f.ks, f.nbatch, F::nw * F::nt * 16);
+    a.kv_blocks = a.k_tiles * a.kv_split * a.kv_heads;
+    if (a.kv_blocks == 0) return;
+    if (a.kv_split == 1) {
+        hipLaunchKernelGGL((attn_dkv_kernel<T, D, F::nw, F::nt, false>), grid_1d(a.kv_blocks), dim3(F::nw * 64), 0, s, a);
+        return;
+    }
+    hipLaunchKernelGGL((attn_dkv_kernel<T, D, F::nw, F::nt, true>), grid_1d(a.kv_blocks), dim3(F::nw * 64), 0, s, a);
+    SumArgs m{};
+    m.part[0] = a.part;
+    m.part[1] = a.part + a.kv_split * f.k_rows * a.kv_heads * D;
+    m.out[0] = a.dk;
+    m.out[1] = a.dv;
+    m.row_stride[0] = a.dk_row;
+    m.row_stride[1] = a.dv_row;
+    m.head_stride[0] = a.dk_head;
+    m.head_stride[1] = a.dv_head;
+    m.offsets = f.ks.offsets;
+    m.rows = f.k_rows;
+    m.heads = a.kv_heads;
+    m.nsplit = a.kv_split;
+    m.nbatch = f.nbatch;
+    launch_sums(m, 2, f.dtype, D, s);
+}
 
 template <typename T, int D>
 hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
-    AttnArgs& f = a.f;
-    if (a.prep_blocks > 0) hipLaunchKernelGGL((attn_prep_kernel<T, D>), grid_1d(a.prep_blocks), dim3(256), 0, s, a);
-    a.k_tiles = (int32_t)tile_count(f.ks, f.nbatch, kBK);
-    a.kv_blocks = a.k_tiles * a.kv_split * a.kv_heads;
-    if (a.kv_blocks > 0) {
-        if (a.kv_split > 1) {
-            hipLaunchKernelGGL((attn_dkv_kernel<T, D, kDkvWaves, kDkvTiles, true>), grid_1d(a.kv_blocks), dim3(kDkvWaves * 64), 0, s, a);
-            SumArgs m{};
-            m.part[0] = a.part;
-            m.part[1] = a.part + a.kv_split * f.k_rows * a.kv_heads * D;
-            m.out[0] = a.dk;
-            m.out[1] = a.dv;
-            m.row_stride[0] = a.dk_row;
-            m.row_stride[1] = a.dv_row;
-            m.head_stride[0] = a.dk_head;
-            m.head_stride[1] = a.dv_head;
-            m.offsets = f.ks.offsets;
-            m.rows = f.k_rows;
-            m.heads = a.kv_heads;
-            m.nsplit = a.kv_split;
-            m.nbatch = f.nbatch;
-            dim3 grid = grid_1d((m.rows * m.heads + 15) / 16);
-            grid.z = 2;
-            hipLaunchKernelGGL((attn_sum_kernel<T, D>), grid, dim3(256), 0, s, m);
-        } else {
-            hipLaunchKernelGGL((attn_dkv_kernel<T, D, kDkvWaves, kDkvTiles, false>), grid_1d(a.kv_blocks), dim3(kDkvWaves * 64), 0, s, a);
-        }
-    }
-    f.q_tiles = (int32_t)tile_count(f.qs, f.nbatch, kBQ);
-    a.q_blocks = f.q_tiles * a.q_split * f.heads;
-    if (a.q_blocks > 0) {
-        if (a.q_split > 1) {
-            hipLaunchKernelGGL((attn_dq_kernel<T, D, kDqWaves, kDqTiles, true>), grid_1d(a.q_blocks), dim3(kDqWaves * 64), 0, s, a);
-            SumArgs m{};
-            m.part[0] = a.part;
-            m.out[0] = a.dq;
-            m.row_stride[0] = a.dq_row;
-            m.head_stride[0] = a.dq_head;
-            m.offsets = f.qs.offsets;
-            m.rows = f.q_rows;
-            m.heads = f.heads;
-            m.nsplit = a.q_split;
-            m.nbatch = f.nbatch;
-            hipLaunchKernelGGL((attn_sum_kernel<T, D>), grid_1d((m.rows * m.heads + 15) / 16), dim3(256), 0, s, m);
-        } else {
-            hipLaunchKernelGGL((attn_dq_kernel<T, D, kDqWaves, kDqTiles, false>), grid_1d(a.q_blocks), dim3(kDqWaves * 64), 0, s, a);
-        }
-    }
+    if (HalfRange<T>::value && a.prep_blocks > 0)
+        hipLaunchKernelGGL((attn_lengths_kernel<T, D>), grid_1d(a.prep_blocks), dim3(256), 0, s, a);
+    if (a.q_small) launch_dq<T, D, Small>(a, s);
+    else launch_dq<T, D, Large>(a, s);
+    if (a.kv_small) launch_dkv<T, D, Small>(a, s);
+    else launch_dkv<T, D, Large>(a, s);
     return hipGetLastError();
 }
 
-int splits(int64_t tiles, int64_t stream, int per) {
-    int64_t n = device_cu_count() / (tiles > 0 ? tiles : 1);
-    if (n > stream / per) n = stream / per;
-    if (n > 64) n = 64;
-    return n < 1 ? 1 : (int)n;
-}
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
@@ -587,10 +613,14 @@ int64_t attn_bwd_plan(AttnBwdArgs& a, void* workspace) {
     AttnArgs& f = a.f;
     a.prep_q_tiles = (int32_t)tile_count(f.qs, f.nbatch, kPrepRows);
     a.prep_k_tiles = (int32_t)tile_count(f.ks, f.nbatch, kPrepRows);
-    a.prep_blocks = a.prep_q_tiles * f.heads + (f.dtype == T2H_F16 ? a.prep_k_tiles * a.kv_heads : 0);
-    const int64_t kt = (f.k_rows / f.nbatch + kBK - 1) / kBK * f.nbatch, qt = (f.q_rows / f.nbatch + kBQ - 1) / kBQ * f.nbatch;
-    a.kv_split = splits(kt * a.kv_heads, f.q_rows / f.nbatch * f.group, 2 * kQT);
-    a.q_split = splits(qt * f.heads, f.k_rows / f.nbatch, 2 * kKT);
+    a.prep_blocks = a.prep_q_tiles * f.heads + a.prep_k_tiles * a.kv_heads;
+    const int64_t gathered = (int64_t)f.qs.share * f.group;     // queries of a key
+    const Plan q = plan_of(f.qs, f.ks.share, f.nbatch, f.heads, false);
+    const Plan kv = plan_of(f.ks, gathered, f.nbatch, a.kv_heads, f.k_lens != nullptr);
+    a.q_small = q.small;
+    a.q_split = q.split;
+    a.kv_small = kv.small;
+    a.kv_split = kv.split;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     int64_t at = 0;
     const auto take = [&](int64_t floats) {
@@ -602,7 +632,9 @@ int64_t attn_bwd_plan(AttnBwdArgs& a, void* workspace) {
     a.lse2 = take(f.q_rows * f.heads);
     a.g_most = take((f.q_rows / kPrepRows + f.nbatch) * f.heads);     // as many with offsets as without
     a.v_most = take((f.k_rows / kPrepRows + f.nbatch) * a.kv_heads);
-    const int64_t pk = a.kv_split > 1 ? 2 * a.kv_split * f.k_rows * a.kv_heads * f.head_dim : 0;
+    // as many with k_lens as without
+    const int64_t kv_most = plan_of(f.ks, gathered, f.nbatch, a.kv_heads, true).split;
+    const int64_t pk = kv_most > 1 ? 2 * kv_most * f.k_rows * a.kv_heads * f.head_dim : 0;
     const int64_t pq = a.q_split > 1 ? a.q_split * f.q_rows * f.heads * f.head_dim : 0;
     a.part = take(pk > pq ? pk : pq);
     return at;
