@@ -7,7 +7,7 @@ CPU tensor raises.
 """
 from __future__ import annotations
 
-import ctypes
+import array
 import functools
 import math
 from typing import Optional, Sequence
@@ -320,29 +320,34 @@ def attn_pack(q=None, k=None, v=None, mp: int = 0, lp: int = 0, bias_q=None, bia
 
 
 # ---- attention -------------------------------------------------------------------
+_current = torch._C._cuda_getDevice if _raw_stream is not None else torch.cuda.current_device
+
+
 def _same_device(ref: torch.Tensor, tensors, what: str) -> None:
     """Every tensor on ref's device, and that the current one (the launch's)."""
     _dev(ref, what)
-    if ref.device.index != torch.cuda.current_device():
+    i = ref.get_device()
+    if i != _current():
         raise ValueError(f"{what}: tensors must be on the current device")
     for t in tensors:
-        if t is not None and t.device != ref.device:
+        if t is not None and t.get_device() != i:
             raise ValueError(f"{what}: tensors are on different devices")
 
 
-def _attn_operand(t: torch.Tensor, rows: int, h: int, d: int, dtype, what: str, name: str):
-    """[rows, H, D] with unit stride on D -> (row stride, head stride) in elements."""
-    if t.dim() != 3 or t.shape != (rows, h, d) or t.dtype != dtype:
-        raise ValueError(f"{what}: {name} must be [{rows}, {h}, {d}] of {dtype}")
-    if t.stride(2) != 1 and t.numel() > 0:
+def _attn_operand(t: torch.Tensor, shape, dtype, what: str, name: str):
+    """[rows, H, D] with unit stride on D -> (row stride, head stride) in
+    elements; 0 for a dimension of one, which has no stride of its own."""
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{what}: {name} must be {list(shape)} of {dtype}")
+    r, h, d = t.stride()
+    if d != 1 and t.numel() > 0:
         raise ValueError(f"{what}: {name} must have unit stride on its last dim")
-    # a dimension of one has no stride of its own
-    return (t.stride(0) if rows > 1 else 0, t.stride(1) if h > 1 else 0)
+    return (r if shape[0] > 1 else 0, h if shape[1] > 1 else 0)
 
 
-def _attn_segments(what: str, nbatch: int, **offsets):
-    for name, t in offsets.items():
-        n = nbatch if name == "k_lens" else nbatch + 1
+def _attn_segments(what: str, nbatch: int, q_offsets, k_offsets, k_lens):
+    for name, t, n in (("q_offsets", q_offsets, nbatch + 1), ("k_offsets", k_offsets, nbatch + 1),
+                       ("k_lens", k_lens, nbatch)):
         if t is not None and (t.dtype != torch.int64 or t.shape != (n,) or not t.is_contiguous()):
             raise ValueError(f"{what}: {name} must be contiguous int64 [{n}]")
 
@@ -350,12 +355,7 @@ def _attn_segments(what: str, nbatch: int, **offsets):
 def _attn_shapes(q, k, what: str):
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"{what}: expected q [rows, H, D] and k, v [rows, Hkv, D]")
-    return *q.shape, k.shape[0], k.shape[1]
-
-
-def _strides_host(pairs):
-    a = (ctypes.c_int64 * (2 * len(pairs)))(*(s for p in pairs for s in p))
-    return a, ctypes.addressof(a)
+    return q.shape, (k.shape[0], k.shape[1], q.shape[2])
 
 
 def _attn_workspace(ws, need: int, device, what: str):
@@ -398,21 +398,19 @@ def attention(q, k, v, scale: Optional[float] = None, q_offsets=None, k_offsets=
     workspace: attention_workspace() bytes (uint8), else allocated here."""
     what = "attention"
     _same_device(q, (k, v, q_offsets, k_offsets, k_lens, out, workspace), what)
-    dt = _dtype(q, what)
-    rows, h, d, krows, kvh = _attn_shapes(q, k, what)
-    _attn_segments(what, nbatch, q_offsets=q_offsets, k_offsets=k_offsets, k_lens=k_lens)
+    dt, qd = _dtype(q, what), q.dtype
+    qs, ks = _attn_shapes(q, k, what)
+    rows, h, d = qs
+    _attn_segments(what, nbatch, q_offsets, k_offsets, k_lens)
     if out is None:
-        out = torch.empty((rows, h, d), dtype=q.dtype, device=q.device)
-    hold, sp = _strides_host((_attn_operand(q, rows, h, d, q.dtype, what, "q"),
-                              _attn_operand(k, krows, kvh, d, q.dtype, what, "k"),
-                              _attn_operand(v, krows, kvh, d, q.dtype, what, "v"),
-                              _attn_operand(out, rows, h, d, q.dtype, what, "out")))
+        out = torch.empty(qs, dtype=qd, device=q.device)
+    strides = array.array("q", (*_attn_operand(q, qs, qd, what, "q"), *_attn_operand(k, ks, qd, what, "k"),
+                                *_attn_operand(v, ks, qd, what, "v"), *_attn_operand(out, qs, qd, what, "out")))
     lse = torch.empty((h, rows), dtype=torch.float32, device=q.device) if need_lse else None
-    ws = _attn_workspace(workspace, attention_workspace(rows, krows, h, kvh, d, nbatch), q.device, what)
-    call("t2h_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), sp, rows, krows, h, kvh,
-         d, dt, d ** -0.5 if scale is None else float(scale), _ptr(q_offsets), _ptr(k_offsets), _ptr(k_lens),
-         int(nbatch), _ptr(ws), ws.numel() if ws is not None else 0, _stream())
-    del hold
+    ws = _attn_workspace(workspace, attention_workspace(rows, ks[0], h, ks[1], d, nbatch), q.device, what)
+    call("t2h_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), strides.buffer_info()[0],
+         rows, ks[0], h, ks[1], d, dt, d ** -0.5 if scale is None else float(scale), _ptr(q_offsets), _ptr(k_offsets),
+         _ptr(k_lens), int(nbatch), _ptr(ws), ws.numel() if ws is not None else 0, _stream())
     return (out, lse) if need_lse else out
 
 
@@ -425,26 +423,31 @@ def attention_backward(dout, q, k, v, out, lse, scale: Optional[float] = None, q
     attention_backward_workspace() bytes (uint8), else allocated here."""
     what = "attention_backward"
     _same_device(q, (dout, k, v, out, lse, q_offsets, k_offsets, k_lens, dq, dk, dv, workspace), what)
-    dt = _dtype(q, what)
-    rows, h, d, krows, kvh = _attn_shapes(q, k, what)
-    _attn_segments(what, nbatch, q_offsets=q_offsets, k_offsets=k_offsets, k_lens=k_lens)
+    dt, qd = _dtype(q, what), q.dtype
+    qs, ks = _attn_shapes(q, k, what)
+    rows, h, d = qs
+    _attn_segments(what, nbatch, q_offsets, k_offsets, k_lens)
     if lse.dtype != torch.float32 or lse.shape != (h, rows) or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be contiguous float32 [{h}, {rows}]")
-    mk = lambda r, n: torch.empty((r, n, d), dtype=q.dtype, device=q.device)
-    dq = mk(rows, h) if dq is None else dq
-    dk = mk(krows, kvh) if dk is None else dk
-    dv = mk(krows, kvh) if dv is None else dv
-    qside = lambda t, name: _attn_operand(t, rows, h, d, q.dtype, what, name)
-    kside = lambda t, name: _attn_operand(t, krows, kvh, d, q.dtype, what, name)
-    hold, sp = _strides_host((qside(q, "q"), kside(k, "k"), kside(v, "v"), qside(out, "out"), qside(dout, "dout"),
-                              qside(dq, "dq"), kside(dk, "dk"), kside(dv, "dv")))
-    ws = _attn_workspace(workspace, attention_backward_workspace(rows, krows, h, kvh, d, nbatch), q.device, what)
+    mk = lambda shape: torch.empty(shape, dtype=qd, device=q.device)
+    dq = mk(qs) if dq is None else dq
+    dk = mk(ks) if dk is None else dk
+    dv = mk(ks) if dv is None else dv
+    strides = array.array("q", (*_attn_operand(q, qs, qd, what, "q"), *_attn_operand(k, ks, qd, what, "k"),
+                                *_attn_operand(v, ks, qd, what, "v"), *_attn_operand(out, qs, qd, what, "out"),
+                                *_attn_operand(dout, qs, qd, what, "dout"), *_attn_operand(dq, qs, qd, what, "dq"),
+                                *_attn_operand(dk, ks, qd, what, "dk"), *_attn_operand(dv, ks, qd, what, "dv")))
+    ws = _attn_workspace(workspace, attention_backward_workspace(rows, ks[0], h, ks[1], d, nbatch), q.device, what)
     call("t2h_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-         dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), sp, rows, krows, h, kvh, d, dt,
-         d ** -0.5 if scale is None else float(scale), _ptr(q_offsets), _ptr(k_offsets), _ptr(k_lens), int(nbatch),
-         _ptr(ws), ws.numel() if ws is not None else 0, _stream())
-    del hold
+         dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), strides.buffer_info()[0], rows, ks[0], h, ks[1],
+         d, dt, d ** -0.5 if scale is None else float(scale), _ptr(q_offsets), _ptr(k_offsets), _ptr(k_lens),
+         int(nbatch), _ptr(ws), ws.numel() if ws is not None else 0, _stream())
     return dq, dk, dv
+
+
+@functools.lru_cache(maxsize=256)
+def _qk_backward_workspace(rows: int, heads: int, head_dim: int, tensors: int) -> int:
+    return int(_lib.load().t2h_qk_rmsnorm_rope_backward_workspace(rows, heads, head_dim, tensors))
 
 
 def qk_rmsnorm_rope_backward(dq=None, dk=None, q=None, k=None, gamma_q=None, gamma_k=None, bias_q=None, bias_k=None,
@@ -479,11 +482,14 @@ def qk_rmsnorm_rope_backward(dq=None, dk=None, q=None, k=None, gamma_q=None, gam
     for t in (gamma_q, gamma_k, bias_q, bias_k):
         if t is not None and (t.dtype != torch.float32 or t.numel() != h * d or not t.is_contiguous()):
             raise ValueError(f"{what}: gamma/bias must be contiguous float32 [H, D]")
-    mk = lambda t: None if t is None else t if in_place else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-    dqi, dki = mk(dq), mk(dk)
-    din_stride = dy_stride if in_place else h * d
-    par = lambda t, g: torch.empty((h, d), dtype=torch.float32, device=ref.device) if t is not None and g is not None else None
-    dgq, dgk, dbq, dbk = par(gamma_q, dq), par(gamma_k, dk), par(bias_q, dq), par(bias_k, dk)
+    if in_place:
+        dqi, dki, din_stride = dq, dk, dy_stride
+    else:
+        dqi, dki = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (dq, dk))
+        din_stride = h * d
+    has = [t is not None and g is not None for t, g in ((gamma_q, dq), (gamma_k, dk), (bias_q, dq), (bias_k, dk))]
+    sums = iter(torch.empty((sum(has), h, d), dtype=torch.float32, device=ref.device).unbind(0) if any(has) else ())
+    dgq, dgk, dbq, dbk = (next(sums) if x else None for x in has)
     hold, fp, fd = _host_freqs(freqs if freqs is not None else [])
     ph_rows = 0
     if phases is not None:
@@ -496,9 +502,8 @@ def qk_rmsnorm_rope_backward(dq=None, dk=None, q=None, k=None, gamma_q=None, gam
             raise ValueError(f"{what}: coords must be contiguous int32 [rows, 1+pos_dim]")
         cc = coords.shape[1]
     ws = workspace
-    if any(t is not None for t in (dgq, dgk, dbq, dbk)):
-        n = (dq is not None) + (dk is not None)
-        need = int(_lib.load().t2h_qk_rmsnorm_rope_backward_workspace(rows, h, d, n))
+    if any(has):
+        need = _qk_backward_workspace(rows, h, d, (dq is not None) + (dk is not None))
         ws = _attn_workspace(ws, max(need, 16), ref.device, what)
     p = _ptr
     call("t2h_qk_rmsnorm_rope_backward", p(q) if dq is not None else None, p(k) if dk is not None else None, p(dq), p(dk),
