@@ -354,7 +354,7 @@ Form form_of(const AttnArgs& a) {
     const int64_t rows = (a.q_rows + a.nbatch - 1) / a.nbatch, cu = device_cu_count();
     if (rows <= 16) return kFew;
     const int64_t per = (int64_t)a.nbatch * a.heads;
-    return (rows + 127) / 128 * per * 2 < cu * 3 ? kSmall : kLarge;
+    return (rows + 127) / 128 * per * 2 < cu * 3 || rows <= 64 ? kSmall : kLarge;
 }
 
 template <typename T, int D, typename F, bool SPLIT>

@@ -355,6 +355,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
                 ++head;
             }
         };
+        const int first = qs.hi - row;
         issue(0);
         if (active) {
             const uint8_t* kb = static_cast<const uint8_t*>(f.k) + (kvh * f.k_head + (int64_t)k0 * f.k_row) * 2;
@@ -365,8 +366,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
                 load_own<T, D>(v[j], vb + 16 * j * f.v_row * 2, k_end - k0 - 16 * j, (uint32_t)f.v_row * 2, lane);
             }
         }
+        int left = first;            // of the tile that is worked on: its rows and those of the head's tiles after it
         for (int it = it0; it < it1; ++it) {
             const int st = (it - it0) & 1;
+            const int rows = left;
+            left = left > kQT ? left - kQT : qs.hi - qs.lo;
             wait_loads<0>();
             wait_lds_reads();
             tile_barrier();
@@ -377,7 +381,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
             const float* ls = reinterpret_cast<const float*>(lds + 4 * kTile) + st * kQT;
             const float* de = ls + 2 * kQT;
 #pragma unroll 1
-            for (int s2 = 0; s2 < kQT / 32; ++s2) {
+            for (int s2 = 0; s2 < kQT / 32 && 32 * s2 < rows; ++s2) {
                 f32x4 s[2][NT], d[2][NT];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -515,7 +519,7 @@ Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads
     const int64_t small = ((int64_t)kept.share + kRowsSmall - 1) / kRowsSmall * per;
     const int64_t most = stream / kSplitRows > 1 ? stream / kSplitRows : 1;
     Plan p{};
-    p.small = large * most * 2 < 3 * cu;
+    p.small = large * most * 2 < 3 * cu || kept.share <= kRowsSmall;
     int64_t n = 1;
     if (p.small) {
         n = cu / (small > 0 ? small : 1);
