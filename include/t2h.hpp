@@ -823,6 +823,116 @@ inline AttnOperands qkv_linear_pack(const Tensor& x, const Tensor& weight, int32
     return p.o;
 }
 
+// Segments of an attention's rows: nbatch equal shares, or device offsets
+// [nbatch + 1] for a side; k_lens (device [nbatch]): only that many keys at the
+// start of a segment count.
+struct Segments {
+    int32_t nbatch = 1;
+    const int64_t* q_offsets = nullptr;
+    const int64_t* k_offsets = nullptr;
+    const int64_t* k_lens = nullptr;
+};
+
+// An attention's output [rows, H, D] and its log-sum-exp [H, rows] (f32).
+struct Attention {
+    Tensor out, lse;
+};
+
+namespace detail {
+
+inline void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const char* what) {
+    if (q.ndim() != 3 || k.ndim() != 3 || k.shape() != v.shape() || q.dim(2) != k.dim(2) || q.dtype() != k.dtype() ||
+        q.dtype() != v.dtype())
+        throw Error(std::string(what) + ": q must be [rows, H, D], k and v [rows, Hkv, D] of one type");
+}
+
+inline Tensor workspace(int64_t bytes) {
+    if (bytes < 0) throw Error(t2h_last_error());
+    return Tensor::empty({(bytes + 3) / 4}, F32);
+}
+
+}  // namespace detail
+
+// softmax(scale * q k^T) v within the segments (t2h_attention): q [rows, H, D],
+// k, v [rows, Hkv, D], f16 or bf16, D 64 or 128; scale 0: 1 / sqrt(D).
+inline Attention attention(const Tensor& q, const Tensor& k, const Tensor& v, float scale = 0.0f,
+                           const Segments& seg = Segments()) {
+    detail::check_attention(q, k, v, "attention");
+    const int32_t h = (int32_t)q.dim(1), kvh = (int32_t)k.dim(1), d = (int32_t)q.dim(2);
+    Attention r{Tensor::empty(q.shape(), q.dtype()), Tensor::empty({q.dim(1), q.dim(0)}, F32)};
+    Tensor ws = detail::workspace(t2h_attention_workspace(q.dim(0), k.dim(0), h, kvh, d, seg.nbatch));
+    check(t2h_attention(q.data(), k.data(), v.data(), r.out.data(), static_cast<float*>(r.lse.data()), nullptr, q.dim(0),
+                        k.dim(0), h, kvh, d, q.dtype(), scale != 0.0f ? scale : 1.0f / std::sqrt((float)d),
+                        seg.q_offsets, seg.k_offsets, seg.k_lens, seg.nbatch, ws.data(), ws.bytes(), nullptr));
+    return r;
+}
+
+// ... on the head-major operands of attn_pack / qkv_linear_pack (k row-major:
+// k_transposed false), whose q holds the scale. rows of the mp / lp are tokens.
+inline Attention attention(const AttnOperands& o, int64_t rows) {
+    if (o.k.ndim() != 3 || o.k.shape() != o.vh.shape() || o.qh.dim(2) != o.k.dim(2))
+        throw Error("attention: k must be row-major [H, lp, D]");
+    const int64_t h = o.qh.dim(0), mp = o.qh.dim(1), lp = o.k.dim(1), d = o.qh.dim(2);
+    if (rows > mp || rows > lp) throw Error("attention: more rows than the operands hold");
+    Attention r{Tensor::empty({rows, h, d}, o.qh.dtype()), Tensor::empty({h, rows}, F32)};
+    const int64_t strides[8] = {d, mp * d, d, lp * d, d, lp * d, h * d, d};
+    Tensor ws = detail::workspace(t2h_attention_workspace(rows, rows, (int32_t)h, (int32_t)h, (int32_t)d, 1));
+    check(t2h_attention(o.qh.data(), o.k.data(), o.vh.data(), r.out.data(), static_cast<float*>(r.lse.data()), strides,
+                        rows, rows, (int32_t)h, (int32_t)h, (int32_t)d, o.qh.dtype(), 1.0f, nullptr, nullptr, nullptr,
+                        1, ws.data(), ws.bytes(), nullptr));
+    return r;
+}
+
+struct AttentionGrads {
+    Tensor dq, dk, dv;
+};
+
+// Gradients of attention() from that of its output (t2h_attention_backward).
+inline AttentionGrads attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
+                                         const Attention& fwd, float scale = 0.0f, const Segments& seg = Segments()) {
+    detail::check_attention(q, k, v, "attention_backward");
+    if (dout.shape() != q.shape() || dout.dtype() != q.dtype() || fwd.out.shape() != q.shape() ||
+        fwd.out.dtype() != q.dtype() || fwd.lse.numel() != q.dim(0) * q.dim(1))
+        throw Error("attention_backward: dout and the forward's results must match q");
+    const int32_t h = (int32_t)q.dim(1), kvh = (int32_t)k.dim(1), d = (int32_t)q.dim(2);
+    AttentionGrads g{Tensor::empty(q.shape(), q.dtype()), Tensor::empty(k.shape(), k.dtype()),
+                     Tensor::empty(v.shape(), v.dtype())};
+    Tensor ws = detail::workspace(t2h_attention_backward_workspace(q.dim(0), k.dim(0), h, kvh, d, seg.nbatch));
+    check(t2h_attention_backward(q.data(), k.data(), v.data(), fwd.out.data(), static_cast<const float*>(fwd.lse.data()),
+                                 dout.data(), g.dq.data(), g.dk.data(), g.dv.data(), nullptr, q.dim(0), k.dim(0), h,
+                                 kvh, d, q.dtype(), scale != 0.0f ? scale : 1.0f / std::sqrt((float)d), seg.q_offsets,
+                                 seg.k_offsets, seg.k_lens, seg.nbatch, ws.data(), ws.bytes(), nullptr));
+    return g;
+}
+
+struct QkGrads {
+    Tensor dx, dgamma, dbias;
+};
+
+// Gradients of one tensor's epilogue (bias, RMS norm with gamma, rotation;
+// t2h_qk_rmsnorm_rope_backward): dy and x [rows, H, D], gamma and bias [H, D]
+// f32 or absent, whose gradients are then absent too.
+inline QkGrads qk_rmsnorm_rope_backward(const Tensor& dy, const Tensor& x, const Tensor& gamma,
+                                        const Tensor& bias = Tensor(), const Rope& rope = Rope()) {
+    if (dy.ndim() != 3 || (x.defined() && (x.shape() != dy.shape() || x.dtype() != dy.dtype())))
+        throw Error("qk_rmsnorm_rope_backward: dy and x must be [rows, H, D] of one type");
+    const int64_t rows = dy.dim(0), h = dy.dim(1), d = dy.dim(2);
+    QkGrads g;
+    g.dx = Tensor::empty(dy.shape(), dy.dtype());
+    if (gamma.defined()) g.dgamma = Tensor::empty({h, d}, F32);
+    if (bias.defined()) g.dbias = Tensor::empty({h, d}, F32);
+    Tensor ws = detail::workspace(t2h_qk_rmsnorm_rope_backward_workspace(rows, (int32_t)h, (int32_t)d, 1));
+    const auto f = [](Tensor& t) { return t.defined() ? static_cast<float*>(t.data()) : nullptr; };
+    check(t2h_qk_rmsnorm_rope_backward(
+        x.defined() ? x.data() : nullptr, nullptr, dy.data(), nullptr, g.dx.data(), nullptr, rows, 0, 0, 0, (int32_t)h,
+        (int32_t)d, dy.dtype(), detail::opt_f32(bias, h * d, "qk_rmsnorm_rope_backward: bias"), nullptr,
+        detail::opt_f32(gamma, h * d, "qk_rmsnorm_rope_backward: gamma"), nullptr, rope.freqs.empty() ? 0 : 1,
+        rope.freqs.empty() ? nullptr : rope.freqs.data(), (int32_t)rope.freqs.size(), 3, nullptr, 0,
+        rope.coords ? rope.coords->data() : nullptr, rope.coords ? (int32_t)rope.coords->cols() : 0, rope.grid_res,
+        f(g.dgamma), nullptr, f(g.dbias), nullptr, ws.data(), ws.bytes(), nullptr));
+    return g;
+}
+
 }  // namespace gpu
 
 // ---- the cross block's per-token glue: gpu/block.mojo:217-397,

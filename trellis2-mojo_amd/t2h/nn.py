@@ -152,6 +152,19 @@ def apply_rotary_embedding(x: torch.Tensor, phases: torch.Tensor) -> torch.Tenso
     return q.reshape(x.shape)
 
 
+def scaled_dot_product_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_lens=None) -> torch.Tensor:
+    """softmax(q k^T / sqrt(D)) v of a dense batch: q [N, L, H, D], k, v [N, Lk,
+    H, D], float16 / bfloat16 (the attention of modules/attention.mojo:110-138);
+    k_lens int64 [N] on the device: only the first k_lens[n] keys count."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("scaled_dot_product_attention: expected [N, L, H, D]")
+    n, l, h, d = q.shape
+    if k.shape[0] != n or k.shape[3] != d:
+        raise ValueError("scaled_dot_product_attention: q/k shape mismatch")
+    flat = lambda t: t.reshape(-1, t.shape[2], d)
+    return ops.attention(flat(q), flat(k), flat(v), nbatch=n, k_lens=k_lens).reshape(q.shape)
+
+
 def _gate(x: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
     """x [N, L, C] * g [N, C] broadcast over L (modules/transformer/modulated.mojo:22-33)."""
     n, l, c = x.shape

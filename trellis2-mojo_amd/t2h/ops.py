@@ -360,28 +360,31 @@ def _attn_shapes(q, k, what: str):
 
 def _attn_workspace(ws, need: int, device, what: str):
     if ws is None:
-        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        return torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
     if ws.dtype != torch.uint8 or not ws.is_contiguous():
         raise ValueError(f"{what}: workspace must be contiguous uint8")
     return ws
 
 
 @functools.lru_cache(maxsize=256)
+def _attn_bytes(name: str, *sizes) -> int:
+    return int(getattr(_lib.load(), name)(*sizes))
+
+
 def attention_workspace(q_rows: int, k_rows: int, heads: int, kv_heads: int, head_dim: int, nbatch: int = 1) -> int:
     """Bytes of workspace with which attention() may split its keys (0: no use for any)."""
-    n = int(_lib.load().t2h_attention_workspace(q_rows, k_rows, heads, kv_heads, head_dim, nbatch))
+    n = _attn_bytes("t2h_attention_workspace", q_rows, k_rows, heads, kv_heads, head_dim, nbatch)
     if n < 0:
-        raise ValueError(_lib.load().t2h_last_error().decode(errors="replace"))
+        raise ValueError("attention_workspace: sizes that attention() does not take")
     return n
 
 
-@functools.lru_cache(maxsize=256)
 def attention_backward_workspace(q_rows: int, k_rows: int, heads: int, kv_heads: int, head_dim: int,
                                  nbatch: int = 1) -> int:
     """Bytes of workspace that attention_backward() needs."""
-    n = int(_lib.load().t2h_attention_backward_workspace(q_rows, k_rows, heads, kv_heads, head_dim, nbatch))
+    n = _attn_bytes("t2h_attention_backward_workspace", q_rows, k_rows, heads, kv_heads, head_dim, nbatch)
     if n < 0:
-        raise ValueError(_lib.load().t2h_last_error().decode(errors="replace"))
+        raise ValueError("attention_backward_workspace: sizes that attention_backward() does not take")
     return n
 
 
@@ -407,7 +410,9 @@ def attention(q, k, v, scale: Optional[float] = None, q_offsets=None, k_offsets=
     strides = array.array("q", (*_attn_operand(q, qs, qd, what, "q"), *_attn_operand(k, ks, qd, what, "k"),
                                 *_attn_operand(v, ks, qd, what, "v"), *_attn_operand(out, qs, qd, what, "out")))
     lse = torch.empty((h, rows), dtype=torch.float32, device=q.device) if need_lse else None
-    ws = _attn_workspace(workspace, attention_workspace(rows, ks[0], h, ks[1], d, nbatch), q.device, what)
+    # sizes that have none are refused by the call
+    ws = _attn_workspace(workspace, _attn_bytes("t2h_attention_workspace", rows, ks[0], h, ks[1], d, nbatch), q.device,
+                         what)
     call("t2h_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), strides.buffer_info()[0],
          rows, ks[0], h, ks[1], d, dt, d ** -0.5 if scale is None else float(scale), _ptr(q_offsets), _ptr(k_offsets),
          _ptr(k_lens), int(nbatch), _ptr(ws), ws.numel() if ws is not None else 0, _stream())
@@ -437,17 +442,13 @@ def attention_backward(dout, q, k, v, out, lse, scale: Optional[float] = None, q
                                 *_attn_operand(v, ks, qd, what, "v"), *_attn_operand(out, qs, qd, what, "out"),
                                 *_attn_operand(dout, qs, qd, what, "dout"), *_attn_operand(dq, qs, qd, what, "dq"),
                                 *_attn_operand(dk, ks, qd, what, "dk"), *_attn_operand(dv, ks, qd, what, "dv")))
-    ws = _attn_workspace(workspace, attention_backward_workspace(rows, ks[0], h, ks[1], d, nbatch), q.device, what)
+    ws = _attn_workspace(workspace, _attn_bytes("t2h_attention_backward_workspace", rows, ks[0], h, ks[1], d, nbatch),
+                         q.device, what)
     call("t2h_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
          dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), strides.buffer_info()[0], rows, ks[0], h, ks[1],
          d, dt, d ** -0.5 if scale is None else float(scale), _ptr(q_offsets), _ptr(k_offsets), _ptr(k_lens),
          int(nbatch), _ptr(ws), ws.numel() if ws is not None else 0, _stream())
     return dq, dk, dv
-
-
-@functools.lru_cache(maxsize=256)
-def _qk_backward_workspace(rows: int, heads: int, head_dim: int, tensors: int) -> int:
-    return int(_lib.load().t2h_qk_rmsnorm_rope_backward_workspace(rows, heads, head_dim, tensors))
 
 
 def qk_rmsnorm_rope_backward(dq=None, dk=None, q=None, k=None, gamma_q=None, gamma_k=None, bias_q=None, bias_k=None,
@@ -503,7 +504,7 @@ def qk_rmsnorm_rope_backward(dq=None, dk=None, q=None, k=None, gamma_q=None, gam
         cc = coords.shape[1]
     ws = workspace
     if any(has):
-        need = _qk_backward_workspace(rows, h, d, (dq is not None) + (dk is not None))
+        need = _attn_bytes("t2h_qk_rmsnorm_rope_backward_workspace", rows, h, d, (dq is not None) + (dk is not None))
         ws = _attn_workspace(ws, max(need, 16), ref.device, what)
     p = _ptr
     call("t2h_qk_rmsnorm_rope_backward", p(q) if dq is not None else None, p(k) if dk is not None else None, p(dq), p(dk),

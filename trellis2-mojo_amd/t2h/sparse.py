@@ -263,3 +263,22 @@ class SparseRotaryPositionEmbedder:
                                      k=kf.reshape(kf.shape[0], -1, self.head_dim), freqs=self.freqs,
                                      pos_dim=self.dim, coords=q.coords, use_rope=True)
         return q.replace(qo.reshape(qf.shape)), k.replace(ko.reshape(kf.shape))
+
+
+def sparse_scaled_dot_product_attention(q, k, v):
+    """Full attention within each batch of a ragged one
+    (sparse/attention/full_attn.mojo): q a SparseTensor or VarLenTensor of feats
+    [T, H, D], k and v of the same batches (feats [Tk, H, D]), or dense [N, L,
+    H, D] tensors (the condition tokens of a cross attention). Returns q's kind."""
+    off = lambda t: t.offsets if isinstance(t, SparseTensor) else t.device_offsets()
+    n = q.batch_size()
+    if isinstance(k, torch.Tensor):
+        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != n:
+            raise ValueError("sparse_scaled_dot_product_attention: k and v must be [N, L, H, D]")
+        kf, vf = (t.reshape(-1, t.shape[2], t.shape[3]) for t in (k, v))
+        ko = None
+    else:
+        if k.batch_size() != n or v.feats.shape != k.feats.shape:
+            raise ValueError("sparse_scaled_dot_product_attention: batch size mismatch")
+        kf, vf, ko = k.feats, v.feats, off(k)
+    return q.replace(ops.attention(q.feats, kf, vf, q_offsets=off(q), k_offsets=ko, nbatch=n))
