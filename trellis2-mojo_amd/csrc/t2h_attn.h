@@ -52,7 +52,8 @@ struct AttnBwdArgs {
     float* lse2;             // [heads, q_rows] log2, less the rounding shift of P
     float* g_most;           // [heads, prep_q_tiles] f16: largest squared row length of dout in each tile
     float* v_most;           // [kv_heads, prep_k_tiles]   ... of v
-    float* part;
+    float* part_kv;          // [2, kv_split, k_rows, kv_heads, head_dim] dk's and dv's parts
+    float* part_q;           // [q_split, q_rows, heads, head_dim]
     int32_t prep_q_tiles, prep_k_tiles, prep_blocks;
     int32_t k_tiles, kv_blocks, q_blocks;   // set by the launcher
 };

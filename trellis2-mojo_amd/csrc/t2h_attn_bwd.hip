@@ -5,10 +5,13 @@
 //   dP_ij = dout_i.v_j                     dS_ij = P_ij (dP_ij - delta_i)
 //   dv_j = sum_i P_ij dout_i    dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i
 //
-// Two launches: dq (and delta) with the queries kept in registers and the keys
-// streaming; dk and dv with the keys kept and the queries streaming. They
-// compute P and dP twice, seven products in place of five, and need no atomic
-// sums, whose order would change the result from run to run.
+// One launch for delta, one for the rest: blocks for dk and dv, which keep their
+// keys in registers while the queries stream past, and blocks for dq, which keep
+// their queries while the keys stream. They compute P and dP twice, seven
+// products in place of five, and need no atomic sums, whose order would change
+// the result from run to run; side by side they fill the GPU where either alone
+// would not (4,096 tokens, 12 heads of 128: 371 -> 355 us; 1,024 tokens, 16 heads of
+// 64: 40.5 -> 29.1).
 //
 // f16: P is rounded as 2^14 P (P is near 1 / keys, below f16's smallest normal
 // number from 16,384 keys on), and dS as 2^e dS, e a power of two from the bound
@@ -41,12 +44,13 @@ __device__ __forceinline__ float shift_ds(float g2, float v2) {
     return (float)e;
 }
 
-// ---- row lengths (f16) ----------------------------------------------------------
-// A block takes up to kPrepRows rows of one segment and one head of dout or of v
-// (only keys that count), 16 lanes a row.
+// ---- delta, and row lengths for f16 ---------------------------------------------
+// A block takes up to kPrepRows rows of one segment and one head of dout and out
+// (or, f16, of v; only keys that count), 16 lanes a row.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_lengths_kernel(AttnBwdArgs a) {
+__global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
     constexpr int E = D / 16;
+    constexpr bool kF16 = HalfRange<T>::value;
     const AttnArgs& f = a.f;
     const int64_t p = block_linear();
     if (p >= a.prep_blocks) return;
@@ -64,7 +68,6 @@ __global__ __launch_bounds__(256) void attn_lengths_kernel(AttnBwdArgs a) {
     }
     const T* x = q ? static_cast<const T*>(a.dout) + head * a.do_head : static_cast<const T*>(f.v) + head * f.v_head;
     const int64_t stride = q ? a.do_row : f.v_row;
-    __shared__ float top[16];
     float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPrepRows / 16; ++i) {
@@ -72,41 +75,55 @@ __global__ __launch_bounds__(256) void attn_lengths_kernel(AttnBwdArgs a) {
         if (row >= s.hi) break;
         float v[E];
         load_elems<T, E>(x + row * stride + m * E, v);
-        most = fmaxf(most, row16_sum(sum_sq_all<E>(v)));
-    }
-    if (m == 0) top[rr] = most;
-    __syncthreads();
-    if (threadIdx.x == 0) {
+        if (kF16) most = fmaxf(most, row16_sum(sum_sq_all<E>(v)));
+        if (q) {
+            float o[E], d = 0.0f;
+            load_elems<T, E>(static_cast<const T*>(f.out) + row * f.o_row + head * f.o_head + m * E, o);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) most = fmaxf(most, top[i]);
-        (q ? a.g_most : a.v_most)[w] = most;
+            for (int e = 0; e < E; ++e) d = fmaf(v[e], o[e], d);
+            d = row16_sum(d);
+            if (m == 0) {
+                const int64_t at = head * f.q_rows + row;
+                const float lse = f.lse[at];
+                a.delta[at] = d;
+                // a row without keys: P = 0
+                a.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e - (kF16 ? kShiftP : 0.0f);
+            }
+        }
+    }
+    if constexpr (kF16) {
+        __shared__ float top[16];
+        if (m == 0) top[rr] = most;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int i = 1; i < 16; ++i) most = fmaxf(most, top[i]);
+            (q ? a.g_most : a.v_most)[w] = most;
+        }
     }
 }
 
 // ---- dq -------------------------------------------------------------------------
 constexpr int kKT = 64;   // keys per tile
 
-template <typename T, int D, int NW, int NT, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnBwdArgs a) {
+template <typename T, int D, int NW, int NT>
+__device__ __forceinline__ void dq_block(const AttnBwdArgs& a, uint8_t* lds, int p) {   // lds: k, k, v, v
     using V8 = typename AttnMma<T>::v8;
     constexpr int BQ = NW * NT * 16;
     constexpr int kTile = kKT * D * 2;
     constexpr bool kF16 = HalfRange<T>::value;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];   // k, k, v, v
     const AttnArgs& f = a.f;
-    const int64_t p = block_linear();
-    if (p >= a.q_blocks) return;
-    const int u = xcd_order((int)p, a.q_blocks);
+    const int u = xcd_order(p, a.q_blocks);
     const int per_head = f.q_tiles * a.q_split;
     const int head = u / per_head;
     const int rem = u - head * per_head;
-    const int split = SPLIT ? rem / f.q_tiles : 0;
+    const int split = rem / f.q_tiles;
     int b;
     const Rows qs = tile_rows<BQ>(f.qs, f.nbatch, rem - split * f.q_tiles, lane_id(), b);
     if (qs.lo >= qs.hi) return;
     Rows ks = segment_keys(f, b);
     const int keys = ks.hi - ks.lo;
-    if constexpr (SPLIT) {
+    if (a.q_split > 1) {
         const int tiles = (ks.hi - ks.lo + kKT - 1) / kKT;
         const int t0 = (int)((int64_t)tiles * split / a.q_split), t1 = (int)((int64_t)tiles * (split + 1) / a.q_split);
         if (t1 < tiles) ks.hi = ks.lo + t1 * kKT;
@@ -143,38 +160,26 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnBwdArgs a) {
         lk.issue(kb, ks.lo, ks.hi, lds);
         lv.issue(vb, ks.lo, ks.hi, lds + 2 * kTile);
     }
-    if (active && (n > 0 || split == 0)) {
+    if (active && n > 0) {
         float v2 = 0.0f;
         if constexpr (kF16) v2 = largest(a.v_most + kvh * a.prep_k_tiles + first_tile<kPrepRows>(f.ks, b), keys, lane);
         const uint8_t* qb = static_cast<const uint8_t*>(f.q) + (head * f.q_head + (int64_t)q0 * f.q_row) * 2;
         const uint8_t* gb = static_cast<const uint8_t*>(a.dout) + (head * a.do_head + (int64_t)q0 * a.do_row) * 2;
-        const uint8_t* ob = static_cast<const uint8_t*>(f.out) + (head * f.o_head + (int64_t)q0 * f.o_row) * 2;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            V8 o[D / 32];
             load_own<T, D>(q[j], qb + 16 * j * f.q_row * 2, qs.hi - q0 - 16 * j, (uint32_t)f.q_row * 2, lane);
             load_own<T, D>(g[j], gb + 16 * j * a.do_row * 2, qs.hi - q0 - 16 * j, (uint32_t)a.do_row * 2, lane);
-            load_own<T, D>(o, ob + 16 * j * f.o_row * 2, qs.hi - q0 - 16 * j, (uint32_t)f.o_row * 2, lane);
             const int row = q0 + 16 * j + r;
-            const float lse = row < qs.hi ? f.lse[head * f.q_rows + row] : -INFINITY;
-            float g2 = 0.0f;
-#pragma unroll
-            for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = (float)g[j][t][e];
-                    de[j] = fmaf(x, (float)o[t][e], de[j]);
-                    if (kF16) g2 = fmaf(x, x, g2);
-                }
-            de[j] += __shfl_xor(de[j], 16);
-            de[j] += __shfl_xor(de[j], 32);
-            // a row without keys: P = 0
-            l2[j] = lse == -INFINITY ? INFINITY : lse * kLog2e - (kF16 ? kShiftP : 0.0f);
-            if (split == 0 && h == 0 && row < qs.hi) {      // for dk and dv
-                a.delta[head * f.q_rows + row] = de[j];
-                a.lse2[head * f.q_rows + row] = l2[j];
+            if (row < qs.hi) {
+                l2[j] = a.lse2[head * f.q_rows + row];
+                de[j] = a.delta[head * f.q_rows + row];
             }
             if constexpr (kF16) {
+                float g2 = 0.0f;
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) g2 = fmaf((float)g[j][t][e], (float)g[j][t][e], g2);
                 g2 += __shfl_xor(g2, 16);
                 g2 += __shfl_xor(g2, 32);
                 const float e = shift_ds(g2, v2);
@@ -258,8 +263,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnBwdArgs a) {
     for (int j = 0; j < NT; ++j) {
         const int row = q0 + 16 * j + r;
         if (row >= qs.hi) continue;
-        if constexpr (SPLIT) {
-            float* po = a.part + (((int64_t)split * f.q_rows + row) * f.heads + head) * D + 4 * h;
+        if (a.q_split > 1) {
+            float* po = a.part_q + (((int64_t)split * f.q_rows + row) * f.heads + head) * D + 4 * h;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(po + 16 * i) = dq[i][j] * w[j];
         } else {
@@ -278,21 +283,18 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(AttnBwdArgs a) {
 // ---- dk, dv ---------------------------------------------------------------------
 constexpr int kQT = 64;   // queries per tile
 
-template <typename T, int D, int NW, int NT, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
+template <typename T, int D, int NW, int NT>
+__device__ __forceinline__ void dkv_block(const AttnBwdArgs& a, uint8_t* lds, int p) {   // lds: q, q, dout, dout, lse2 x 2, delta x 2
     using V8 = typename AttnMma<T>::v8;
     constexpr int BK = NW * NT * 16;
     constexpr int kTile = kQT * D * 2;
     constexpr bool kF16 = HalfRange<T>::value;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile + 4 * kQT * 4];   // q, q, dout, dout, lse2 x 2, delta x 2
     const AttnArgs& f = a.f;
-    const int64_t p = block_linear();
-    if (p >= a.kv_blocks) return;
-    const int u = xcd_order((int)p, a.kv_blocks);
+    const int u = xcd_order(p, a.kv_blocks);
     const int per_head = a.k_tiles * a.kv_split;
     const int kvh = u / per_head;
     const int rem = u - kvh * per_head;
-    const int split = SPLIT ? rem / a.k_tiles : 0;
+    const int split = rem / a.k_tiles;
     int b;
     const Rows ks = tile_rows<BK>(f.ks, f.nbatch, rem - split * a.k_tiles, lane_id(), b);
     if (ks.lo >= ks.hi) return;
@@ -307,8 +309,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
     const bool active = k0 < k_end;
     const int tiles = (qs.hi - qs.lo + kQT - 1) / kQT;
     const int total = ks.lo < k_end ? tiles * f.group : 0;
-    const int it0 = SPLIT ? (int)((int64_t)total * split / a.kv_split) : 0;
-    const int it1 = SPLIT ? (int)((int64_t)total * (split + 1) / a.kv_split) : total;
+    const int it0 = (int)((int64_t)total * split / a.kv_split);
+    const int it1 = (int)((int64_t)total * (split + 1) / a.kv_split);
 
     TileLoad<D, kQT, NW> lq, lg;
     lq.init(wave, lane, f.q_row);
@@ -335,7 +337,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
         }
         // the next tile: query head and first row
         int head = kvh * f.group, row = qs.lo;
-        if constexpr (SPLIT) {
+        if (it0 > 0) {
             head += it0 / tiles;
             row += it0 % tiles * kQT;
         }
@@ -443,8 +445,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
         const int row = k0 + 16 * j + r;
         if (row >= ks.hi) continue;
         const bool counts = row < k_end;
-        if constexpr (SPLIT) {
-            float* pk = a.part + (((int64_t)split * f.k_rows + row) * a.kv_heads + kvh) * D + 4 * h;
+        if (a.kv_split > 1) {
+            float* pk = a.part_kv + (((int64_t)split * f.k_rows + row) * a.kv_heads + kvh) * D + 4 * h;
             float* pv = pk + (int64_t)a.kv_split * f.k_rows * a.kv_heads * D;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
@@ -468,6 +470,15 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkv_kernel(AttnBwdArgs a) {
             }
         }
     }
+}
+
+// Blocks for dk and dv first: they take longer.
+template <typename T, int D, int KV, int Q>
+__global__ __launch_bounds__(256, 2) void attn_bwd_kernel(AttnBwdArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kQT * D * 2 + 4 * kQT * 4];
+    const int64_t p = block_linear();
+    if (p < a.kv_blocks) dkv_block<T, D, 4, KV>(a, lds, (int)p);
+    else if (p - a.kv_blocks < a.q_blocks) dq_block<T, D, 4, Q>(a, lds, (int)(p - a.kv_blocks));
 }
 
 // Sum of the parts [nsplit, rows, heads, D] in order; blockIdx.z: part set
@@ -499,21 +510,20 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(SumArgs a) {
     store_elems<T, E>(static_cast<T*>(a.out[w]) + row * a.row_stride[w] + head * a.head_stride[w] + m * E, acc);
 }
 
-// The kernels' forms: waves and 16-token tiles a wave. Four waves, two blocks a
-// CU.
-struct Large { static constexpr int nw = 4, nt = 2; };
-struct Small { static constexpr int nw = 4, nt = 1; };
+// Four waves a block, two blocks a CU; a wave keeps two 16-token tiles (the large
+// form) or one (the small).
 constexpr int kRowsLarge = 128, kRowsSmall = 64;   // tokens a block keeps
 constexpr int kSplitRows = 1024;                   // streaming tokens that a part of the large form has at least
 
 // How one side's blocks take their work: the large form, its streaming side in as
-// many parts as the GPU's two blocks a CU take at once (39,804 queries of 1,029
-// keys, k_lens: dk, dv in 1 part and the rest of the pass 1,156 us, 2: 824, 3: 700, 4: 821;
-// 8,192 queries, all keys: 3 parts 174 us, 4: 141, 5: 185); where the parts would
-// be too short for 1.5 blocks a CU, the small form. padded: of the blocks' own
-// tokens only some count, three in four say.
+// many parts as the GPU's two blocks a CU take at once (dk, dv of 1,029 keys, 12
+// heads of 128, the whole pass: 8,192 queries in 2 parts 229 us, 4: 214, 6: 221; 2 x
+// 19,902 queries in 2 parts 677 us, 3: 692, 6: 718); where the parts would be too
+// short for 1.5 blocks a CU (300 queries, 3,000 keys: large 57.6 us, small 51.5),
+// and for segments no longer than its tile (64 of 37 tokens, 16 heads of 64, each
+// side's blocks alone: 12.2 and 12.5 us, small 8.5 and 9.9), the small form.
 struct Plan { bool small; int split; };
-Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads, bool padded) {
+Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads) {
     const int64_t cu = device_cu_count(), per = (int64_t)nbatch * heads;
     const int64_t large = ((int64_t)kept.share + kRowsLarge - 1) / kRowsLarge * per;
     const int64_t small = ((int64_t)kept.share + kRowsSmall - 1) / kRowsSmall * per;
@@ -525,85 +535,65 @@ Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads
         n = cu / (small > 0 ? small : 1);
         if (n > stream / 128) n = stream / 128;
     } else if (large * 2 < 3 * cu) {
-        n = 2 * cu * (padded ? 4 : 3) / (large * 3);
+        n = 2 * cu / large;
         if (n > most) n = most;
     }
     p.split = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     return p;
 }
 
-void launch_sums(const SumArgs& m, int sets, int32_t dtype, int32_t head_dim, hipStream_t s) {
+template <typename T, int D>
+void launch_sums(const SumArgs& m, int sets, hipStream_t s) {
     dim3 grid = grid_1d((m.rows * m.heads + 15) / 16);
     grid.z = sets;
-    if (dtype == T2H_F16) {
-        if (head_dim == 128) hipLaunchKernelGGL((attn_sum_kernel<_Float16, 128>), grid, dim3(256), 0, s, m);
-        else hipLaunchKernelGGL((attn_sum_kernel<_Float16, 64>), grid, dim3(256), 0, s, m);
-    } else {
-        if (head_dim == 128) hipLaunchKernelGGL((attn_sum_kernel<__bf16, 128>), grid, dim3(256), 0, s, m);
-        else hipLaunchKernelGGL((attn_sum_kernel<__bf16, 64>), grid, dim3(256), 0, s, m);
-    }
+    hipLaunchKernelGGL((attn_sum_kernel<T, D>), grid, dim3(256), 0, s, m);
 }
 
-template <typename T, int D, typename F>
-void launch_dq(AttnBwdArgs& a, hipStream_t s) {
+template <typename T, int D, int KV, int Q>
+void launch_forms(AttnBwdArgs& a, hipStream_t s) {
     AttnArgs& f = a.f;
-    f.q_tiles = (int32_t)tile_count(f.qs, f.nbatch, F::nw * F::nt * 16);
-    a.q_blocks = f.q_tiles * a.q_split * f.heads;
-    if (a.q_blocks == 0) return;
-    if (a.q_split == 1) {
-        hipLaunchKernelGGL((attn_dq_kernel<T, D, F::nw, F::nt, false>), grid_1d(a.q_blocks), dim3(F::nw * 64), 0, s, a);
-        return;
-    }
-    hipLaunchKernelGGL((attn_dq_kernel<T, D, F::nw, F::nt, true>), grid_1d(a.q_blocks), dim3(F::nw * 64), 0, s, a);
-    SumArgs m{};
-    m.part[0] = a.part;
-    m.out[0] = a.dq;
-    m.row_stride[0] = a.dq_row;
-    m.head_stride[0] = a.dq_head;
-    m.offsets = f.qs.offsets;
-    m.rows = f.q_rows;
-    m.heads = f.heads;
-    m.nsplit = a.q_split;
-    m.nbatch = f.nbatch;
-    launch_sums(m, 1, f.dtype, D, s);
-}
-
-template <typename T, int D, typename F>
-void launch_dkv(AttnBwdArgs& a, hipStream_t s) {
-    const AttnArgs& f = a.f;
-    a.k_tiles = (int32_t)tile_count(f.ks, f.nbatch, F::nw * F::nt * 16);
+    a.k_tiles = (int32_t)tile_count(f.ks, f.nbatch, KV * 64);
+    f.q_tiles = (int32_t)tile_count(f.qs, f.nbatch, Q * 64);
     a.kv_blocks = a.k_tiles * a.kv_split * a.kv_heads;
-    if (a.kv_blocks == 0) return;
-    if (a.kv_split == 1) {
-        hipLaunchKernelGGL((attn_dkv_kernel<T, D, F::nw, F::nt, false>), grid_1d(a.kv_blocks), dim3(F::nw * 64), 0, s, a);
-        return;
-    }
-    hipLaunchKernelGGL((attn_dkv_kernel<T, D, F::nw, F::nt, true>), grid_1d(a.kv_blocks), dim3(F::nw * 64), 0, s, a);
-    SumArgs m{};
-    m.part[0] = a.part;
-    m.part[1] = a.part + a.kv_split * f.k_rows * a.kv_heads * D;
-    m.out[0] = a.dk;
-    m.out[1] = a.dv;
-    m.row_stride[0] = a.dk_row;
-    m.row_stride[1] = a.dv_row;
-    m.head_stride[0] = a.dk_head;
-    m.head_stride[1] = a.dv_head;
-    m.offsets = f.ks.offsets;
-    m.rows = f.k_rows;
-    m.heads = a.kv_heads;
-    m.nsplit = a.kv_split;
-    m.nbatch = f.nbatch;
-    launch_sums(m, 2, f.dtype, D, s);
+    a.q_blocks = f.q_tiles * a.q_split * f.heads;
+    const int64_t blocks = (int64_t)a.kv_blocks + a.q_blocks;
+    if (blocks > 0) hipLaunchKernelGGL((attn_bwd_kernel<T, D, KV, Q>), grid_1d(blocks), dim3(256), 0, s, a);
 }
 
 template <typename T, int D>
 hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
-    if (HalfRange<T>::value && a.prep_blocks > 0)
-        hipLaunchKernelGGL((attn_lengths_kernel<T, D>), grid_1d(a.prep_blocks), dim3(256), 0, s, a);
-    if (a.q_small) launch_dq<T, D, Small>(a, s);
-    else launch_dq<T, D, Large>(a, s);
-    if (a.kv_small) launch_dkv<T, D, Small>(a, s);
-    else launch_dkv<T, D, Large>(a, s);
+    const AttnArgs& f = a.f;
+    if (a.prep_blocks > 0) hipLaunchKernelGGL((attn_prep_kernel<T, D>), grid_1d(a.prep_blocks), dim3(256), 0, s, a);
+    if (a.kv_small) a.q_small ? launch_forms<T, D, 1, 1>(a, s) : launch_forms<T, D, 1, 2>(a, s);
+    else a.q_small ? launch_forms<T, D, 2, 1>(a, s) : launch_forms<T, D, 2, 2>(a, s);
+    SumArgs m{};
+    m.nbatch = f.nbatch;
+    if (a.kv_split > 1 && a.kv_blocks > 0) {
+        m.part[0] = a.part_kv;
+        m.part[1] = a.part_kv + a.kv_split * f.k_rows * a.kv_heads * D;
+        m.out[0] = a.dk;
+        m.out[1] = a.dv;
+        m.row_stride[0] = a.dk_row;
+        m.row_stride[1] = a.dv_row;
+        m.head_stride[0] = a.dk_head;
+        m.head_stride[1] = a.dv_head;
+        m.offsets = f.ks.offsets;
+        m.rows = f.k_rows;
+        m.heads = a.kv_heads;
+        m.nsplit = a.kv_split;
+        launch_sums<T, D>(m, 2, s);
+    }
+    if (a.q_split > 1 && a.q_blocks > 0) {
+        m.part[0] = a.part_q;
+        m.out[0] = a.dq;
+        m.row_stride[0] = a.dq_row;
+        m.head_stride[0] = a.dq_head;
+        m.offsets = f.qs.offsets;
+        m.rows = f.q_rows;
+        m.heads = f.heads;
+        m.nsplit = a.q_split;
+        launch_sums<T, D>(m, 1, s);
+    }
     return hipGetLastError();
 }
 
@@ -612,15 +602,14 @@ int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 }  // namespace
 
 // The workspace: delta and lse2 [heads, q_rows], the maxima (f16), then the
-// parts of whichever of dk, dv and dq are split (one after the other).
+// parts of whichever of dk, dv and dq are split.
 int64_t attn_bwd_plan(AttnBwdArgs& a, void* workspace) {
     AttnArgs& f = a.f;
     a.prep_q_tiles = (int32_t)tile_count(f.qs, f.nbatch, kPrepRows);
     a.prep_k_tiles = (int32_t)tile_count(f.ks, f.nbatch, kPrepRows);
-    a.prep_blocks = a.prep_q_tiles * f.heads + a.prep_k_tiles * a.kv_heads;
-    const int64_t gathered = (int64_t)f.qs.share * f.group;     // queries of a key
-    const Plan q = plan_of(f.qs, f.ks.share, f.nbatch, f.heads, false);
-    const Plan kv = plan_of(f.ks, gathered, f.nbatch, a.kv_heads, f.k_lens != nullptr);
+    a.prep_blocks = a.prep_q_tiles * f.heads + (f.dtype == T2H_F16 ? a.prep_k_tiles * a.kv_heads : 0);
+    const Plan q = plan_of(f.qs, f.ks.share, f.nbatch, f.heads);
+    const Plan kv = plan_of(f.ks, (int64_t)f.qs.share * f.group, f.nbatch, a.kv_heads);
     a.q_small = q.small;
     a.q_split = q.split;
     a.kv_small = kv.small;
@@ -636,11 +625,10 @@ int64_t attn_bwd_plan(AttnBwdArgs& a, void* workspace) {
     a.lse2 = take(f.q_rows * f.heads);
     a.g_most = take((f.q_rows / kPrepRows + f.nbatch) * f.heads);     // as many with offsets as without
     a.v_most = take((f.k_rows / kPrepRows + f.nbatch) * a.kv_heads);
-    // as many with k_lens as without
-    const int64_t kv_most = plan_of(f.ks, gathered, f.nbatch, a.kv_heads, true).split;
-    const int64_t pk = kv_most > 1 ? 2 * kv_most * f.k_rows * a.kv_heads * f.head_dim : 0;
-    const int64_t pq = a.q_split > 1 ? a.q_split * f.q_rows * f.heads * f.head_dim : 0;
-    a.part = take(pk > pq ? pk : pq);
+    const int64_t pk = a.kv_split > 1 ? 2 * (int64_t)a.kv_split * f.k_rows * a.kv_heads * f.head_dim : 0;
+    const int64_t pq = a.q_split > 1 ? (int64_t)a.q_split * f.q_rows * f.heads * f.head_dim : 0;
+    a.part_kv = take(pk);
+    a.part_q = take(pq);
     return at;
 }
 
