@@ -20,6 +20,9 @@ __global__ __launch_bounds__(NW * KG * 64, 2) void attn_kernel(AttnArgs a) {
     using V8 = typename AttnMma<T>::v8;
     constexpr int BQ = NW * NT * 16, BK = KG * KT, kS = KT / 16, kP = KT / 32;
     constexpr int kTile = KT * D * 2, kStage = KG * kTile;
+    // Few queries wait for memory, not for the matrix cores: there the
+    // probabilities keep twice the type's bits, as two products.
+    constexpr bool FINE = KG > 1;
     constexpr float kRise = 8.0f;   // the reference follows the maximum once it is this far above (log2)
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kStage];   // K, K, V, V
     const int64_t p = block_linear();
@@ -173,7 +176,10 @@ __global__ __launch_bounds__(NW * KG * 64, 2) void attn_kernel(AttnArgs a) {
                 for (int i = 0; i < D / 16; ++i) {
                     const V8 f = tr_frag<T, D>(vt, fa.tr, k2, i);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) o[i][j] = AttnMma<T>::run(f, pf[j][k2], o[i][j]);
+                    for (int j = 0; j < NT; ++j) {
+                        o[i][j] = AttnMma<T>::run(f, pf[j][k2], o[i][j]);
+                        if constexpr (FINE) o[i][j] = AttnMma<T>::run(f, rest_frag<T>(s[2 * k2][j], s[2 * k2 + 1][j], pf[j][k2]), o[i][j]);
+                    }
                 }
             if (MORE) {
                 tops(sn, top);

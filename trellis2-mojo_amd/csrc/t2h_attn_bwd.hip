@@ -255,6 +255,11 @@ __device__ __forceinline__ void dq_block(const AttnBwdArgs& a, uint8_t* lds, int
 #pragma unroll
                     for (int j = 0; j < NT; ++j) dq[i][j] = AttnMma<T>::run(x, df[j], dq[i][j]);
                 }
+                if (NT == 1 && a.fine) {
+                    const V8 rest = rest_frag<T>(d[0][0], d[1][0], df[0]);
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) dq[i][0] = AttnMma<T>::run(tr_frag<T, D>(kt, fa.tr, s2, i), rest, dq[i][0]);
+                }
             }
         }
     }
@@ -436,6 +441,14 @@ __device__ __forceinline__ void dkv_block(const AttnBwdArgs& a, uint8_t* lds, in
 #pragma unroll
                     for (int j = 0; j < NT; ++j) dk[i][j] = AttnMma<T>::run(x, df[j], dk[i][j]);
                 }
+                if (NT == 1 && a.fine) {
+                    const V8 pr = rest_frag<T>(s[0][0], s[1][0], pf[0]), dr = rest_frag<T>(d[0][0], d[1][0], df[0]);
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        dv[i][0] = AttnMma<T>::run(tr_frag<T, D>(gt, fa.tr, s2, i), pr, dv[i][0]);
+                        dk[i][0] = AttnMma<T>::run(tr_frag<T, D>(qt, fa.tr, s2, i), dr, dk[i][0]);
+                    }
+                }
             }
         }
     }
@@ -513,6 +526,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(SumArgs a) {
 // Four waves a block, two blocks a CU; a wave keeps two 16-token tiles (the large
 // form) or one (the small).
 constexpr int kRowsLarge = 128, kRowsSmall = 64;   // tokens a block keeps
+constexpr int kFine = 64;                          // tokens
 constexpr int kSplitRows = 1024;                   // streaming tokens that a part of the large form has at least
 
 // How one side's blocks take their work: the large form, its streaming side in as
@@ -522,14 +536,19 @@ constexpr int kSplitRows = 1024;                   // streaming tokens that a pa
 // short for 1.5 blocks a CU (300 queries, 3,000 keys: large 57.6 us, small 51.5),
 // and for segments no longer than its tile (64 of 37 tokens, 16 heads of 64, each
 // side's blocks alone: 12.2 and 12.5 us, small 8.5 and 9.9), the small form.
+// Few queries or few keys (kFine in all): P and dS keep twice the type's bits, as
+// two products. Such calls wait for memory, not for the matrix cores, and in their
+// results a few terms of a sum weigh most, whose rounding does not average out
+// (one query, 10,474 keys, f16: dk 3.4e-4 off in the 2-norm, 2.2e-4 so, of which
+// 2.1e-4 is its own rounding; 16 queries, 60,000 keys 323 -> 381 us).
 struct Plan { bool small; int split; };
-Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads) {
+Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads, bool fine) {
     const int64_t cu = device_cu_count(), per = (int64_t)nbatch * heads;
     const int64_t large = ((int64_t)kept.share + kRowsLarge - 1) / kRowsLarge * per;
     const int64_t small = ((int64_t)kept.share + kRowsSmall - 1) / kRowsSmall * per;
     const int64_t most = stream / kSplitRows > 1 ? stream / kSplitRows : 1;
     Plan p{};
-    p.small = large * most * 2 < 3 * cu || kept.share <= kRowsSmall;
+    p.small = large * most * 2 < 3 * cu || kept.share <= kRowsSmall || fine;
     int64_t n = 1;
     if (p.small) {
         n = cu / (small > 0 ? small : 1);
@@ -608,11 +627,13 @@ int64_t attn_bwd_plan(AttnBwdArgs& a, void* workspace) {
     a.prep_q_tiles = (int32_t)tile_count(f.qs, f.nbatch, kPrepRows);
     a.prep_k_tiles = (int32_t)tile_count(f.ks, f.nbatch, kPrepRows);
     a.prep_blocks = a.prep_q_tiles * f.heads + (f.dtype == T2H_F16 ? a.prep_k_tiles * a.kv_heads : 0);
-    const Plan q = plan_of(f.qs, f.ks.share, f.nbatch, f.heads);
-    const Plan kv = plan_of(f.ks, (int64_t)f.qs.share * f.group, f.nbatch, a.kv_heads);
+    const bool fine = f.q_rows <= kFine || f.k_rows <= kFine;
+    const Plan q = plan_of(f.qs, f.ks.share, f.nbatch, f.heads, fine);
+    const Plan kv = plan_of(f.ks, (int64_t)f.qs.share * f.group, f.nbatch, a.kv_heads, fine);
     a.q_small = q.small;
     a.q_split = q.split;
     a.kv_small = kv.small;
+    a.fine = fine;
     a.kv_split = kv.split;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     int64_t at = 0;

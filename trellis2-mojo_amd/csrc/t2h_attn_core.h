@@ -256,6 +256,19 @@ __device__ __forceinline__ float sum_sq_all(const float (&x)[N]) {
     return s;
 }
 
+// What that rounding loses, rounded in turn: the two together hold twice the bits.
+template <typename T>
+__device__ __forceinline__ typename AttnMma<T>::v8 rest_frag(const f32x4& a, const f32x4& b,
+                                                             const typename AttnMma<T>::v8& v) {
+    typename AttnMma<T>::v8 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = (T)(a[i] - (float)v[i]);
+        w[4 + i] = (T)(b[i] - (float)v[4 + i]);
+    }
+    return w;
+}
+
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.69314718055994531f;
 // 2^x: v_exp_f32 (results below 2^-126 are zero).
