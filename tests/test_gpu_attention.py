@@ -391,3 +391,21 @@ def test_offsets_far_below_zero_stay_inside(dev):
     o2, l2 = ops.attention(q, k, v, need_lse=True)
     for a, b in zip(got, (o2, l2, *ops.attention_backward(g, q, k, v, o2, l2))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 16, 40])
+def test_nan_keys_that_fill_a_part_of_a_tile(dev, rows, d):
+    """Keys are dealt out to waves: a wave whose scores are all NaN is no wave without keys."""
+    from t2h import ops
+
+    for bad in (slice(32, 64), slice(0, 32), slice(40, 41), slice(96, 130), slice(0, 1024)):
+        for krows in (130, 1024):
+            q, k, v, _ = make(9, rows, krows, 2, 2, d, F16, dev)
+            k[bad] = math.nan
+            out, lse = ops.attention(q, k, v, need_lse=True)
+            assert out.isnan().all() and lse.isnan().all(), (bad, krows)
+    q, k, v, _ = make(9, rows, 5000, 2, 2, d, F16, dev)      # and in a split's part
+    k[2048:2112] = math.nan
+    out, lse = ops.attention(q, k, v, need_lse=True)
+    assert out.isnan().all() and lse.isnan().all()

@@ -235,7 +235,7 @@ __global__ __launch_bounds__(NW * KG * 64, 2) void attn_kernel(AttnArgs a) {
             for (int j = 0; j < NT; ++j) {
                 const float* m = pm + ((at * NT + j) * 64 + lane) * 3;
                 const float m1 = m[0], t1 = m[1], l1 = m[2];
-                if (t1 == -INFINITY) continue;      // a group without keys
+                if (t1 == -INFINITY && l1 == 0.0f) continue;      // a group without keys (its sum is NaN where its scores are)
                 const float top = thr[j] == -INFINITY ? m1 : fmaxf(mc[j], m1);
                 const float w0 = thr[j] == -INFINITY ? 0.0f : exp2_f(mc[j] - top), w1 = exp2_f(m1 - top);
                 mc[j] = top;
