@@ -220,7 +220,7 @@ int32_t t2h_attn_pack(const void* q, const void* k, const void* v,
  * contiguous), so that the operands can be views of a packed qkv [rows, 3, H,
  * D] (row 3HD, head D) or the head-major outputs of t2h_attn_pack /
  * t2h_qkv_linear_pack (row D, head mp * D; qh holds the scale: pass 1); NULL =
- * all contiguous. Multiples of 8, rows at most 2^23; 16-byte aligned tensors.
+ * all contiguous. Multiples of 8, rows at most 2^22; 16-byte aligned tensors.
  * Segments: nbatch of them, rows [offsets[b], offsets[b + 1]) (int64 device
  * [nbatch + 1]) or equal shares where a side's offsets are NULL. k_lens (int64
  * device [nbatch] or NULL): only that many keys at the start of a segment

@@ -56,7 +56,7 @@ def test_attention_refuses(lib, call, args, code, text):
 
 @pytest.mark.parametrize("i,name", enumerate(["q", "k", "v", "out", "dout", "dq", "dk", "dv"]))
 @pytest.mark.parametrize("bad,code", [((60, 64), -1), ((256, 4), -1), ((-256, 64), -1), ((256, -64), -1),
-                                      ((260, 64), -1), ((256, 68), -1), ((1 << 24, 64), -2)])
+                                      ((260, 64), -1), ((256, 68), -1), ((1 << 24, 64), -2), (((1 << 22) + 8, 64), -2)])
 def test_attention_refuses_strides(lib, i, name, bad, code):
     st = [256, 64] * 8
     st[2 * i:2 * i + 2] = bad

@@ -409,3 +409,17 @@ def test_nan_keys_that_fill_a_part_of_a_tile(dev, rows, d):
     k[2048:2112] = math.nan
     out, lse = ops.attention(q, k, v, need_lse=True)
     assert out.isnan().all() and lse.isnan().all()
+
+
+@pytest.mark.parametrize("rows,d", [(1, 64), (5, 128), (64, 64)])
+def test_rows_far_apart(dev, rows, d):
+    """The largest row stride: a tile's last row is 2^31 bytes from its first."""
+    from t2h import ops
+
+    stride, n = 1 << 22, 300
+    q, k, v, g = make(3, rows, n, 1, 1, d, BF16, dev)
+    big = torch.empty(((n - 1) * stride + 2 * d,), dtype=BF16, device=dev)
+    kk, vv = (big.as_strided((n, 1, d), (stride, d, 1), at).copy_(t) for at, t in ((0, k), (d, v)))
+    out, lse, _ = run_both(q, kk, vv, g, d ** -0.5, dev)
+    again, _ = ops.attention(q, k, v, scale=d ** -0.5, need_lse=True)
+    assert torch.equal(out, again)

@@ -511,8 +511,9 @@ int32_t t2h_qk_rmsnorm_rope_backward(const void* q_in, const void* k_in, const v
 namespace t2h {
 namespace {
 
-// Row strides reach 64 rows on in 32-bit byte offsets.
-constexpr int64_t kAttnMaxRowStride = int64_t(1) << 23;
+// A tile's 32-bit byte offsets stay below 2^31: 256 rows at most (the forward's
+// eight key groups of 32).
+constexpr int64_t kAttnMaxRowStride = int64_t(1) << 22;
 
 int32_t attn_sizes(const char* fn, int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
                    int32_t nbatch) {
@@ -545,7 +546,7 @@ int32_t attn_tensor(const char* fn, const char* name, const void* p, int64_t row
     if (rows > 0 && p == nullptr) return fail(T2H_EINVAL, "%s: %s is NULL", fn, name);
     if (row < head_dim || head < head_dim || row % 8 != 0 || head % 8 != 0)
         return fail(T2H_EINVAL, "%s: %s strides must be multiples of 8 elements, at least head_dim", fn, name);
-    if (row > kAttnMaxRowStride) return fail(T2H_EUNSUPPORTED, "%s: %s row stride above 2^23 elements", fn, name);
+    if (row > kAttnMaxRowStride) return fail(T2H_EUNSUPPORTED, "%s: %s row stride above 2^22 elements", fn, name);
     if (!aligned(p, 16)) return fail(T2H_EINVAL, "%s: %s must be 16-byte aligned", fn, name);
     return T2H_OK;
 }
