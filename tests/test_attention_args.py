@@ -77,6 +77,25 @@ def test_attention_refuses_aliases_and_workspaces(lib):
     assert bwd(lib, ws=ctypes.c_void_p(24)) == -1 and b"16-byte aligned" in lib.t2h_last_error()
 
 
+def test_expanded_tensors_are_refused(monkeypatch):
+    """A stride of 0 means contiguous to the C ABI: it would read past an
+    expanded tensor's end. A dimension of one has no stride that counts."""
+    full, one = torch.zeros((6, 2, 64)), torch.zeros((1, 1, 64))
+    rows, heads = torch.zeros((1, 2, 64)).expand(6, 2, 64), torch.zeros((6, 1, 64)).expand(6, 2, 64)
+    for bad in (rows, heads):
+        with pytest.raises(ValueError, match="x must not be expanded"):
+            ops._attn_operand(bad, bad.shape, bad.dtype, "f", "x")
+    assert ops._attn_operand(full, full.shape, full.dtype, "f", "x") == (128, 64)
+    assert ops._attn_operand(one.expand(1, 1, 64), one.shape, one.dtype, "f", "x") == (0, 0)
+    monkeypatch.setattr(ops, "_dev", lambda *a: None)
+    with pytest.raises(ValueError, match="rows must not overlap"):
+        ops._heads_view(rows, "f")
+    with pytest.raises(ValueError, match="heads must be contiguous"):
+        ops._heads_view(heads, "f")
+    assert ops._heads_view(full, "f") == (6, 2, 64, 128)
+    assert ops._heads_view(torch.zeros((7, 64)).as_strided((1, 2, 64), (0, 64, 1)), "f") == (1, 2, 64, 128)
+
+
 def test_attention_workspaces(lib):
     assert lib.t2h_attention_workspace(-1, 1, 1, 1, 64, 1) == -1
     assert lib.t2h_attention_workspace(1, 1, 1, 1, 60, 1) == -1

@@ -423,3 +423,19 @@ def test_rows_far_apart(dev, rows, d):
     out, lse, _ = run_both(q, kk, vv, g, d ** -0.5, dev)
     again, _ = ops.attention(q, k, v, scale=d ** -0.5, need_lse=True)
     assert torch.equal(out, again)
+
+
+def test_expanded_gradients_are_refused(dev):
+    from t2h import ops
+
+    q, k, v, g = make(3, 20, 20, 2, 2, 64, F16, dev)
+    out, lse = ops.attention(q, k, v, need_lse=True)
+    for bad in (g[:1].expand(20, 2, 64), g[:, :1].expand(20, 2, 64)):
+        with pytest.raises(ValueError, match="must not be expanded"):
+            ops.attention_backward(bad, q, k, v, out, lse)
+        with pytest.raises(ValueError, match="must not be expanded"):
+            ops.attention(bad, k, v)
+    with pytest.raises(ValueError, match="unit stride"):
+        ops.attention_backward(g[:, :, :1].expand(20, 2, 64), q, k, v, out, lse)
+    with pytest.raises(ValueError, match="rows must not overlap"):
+        ops.qk_rmsnorm_rope_backward(dq=g[:1].expand(20, 2, 64), use_rope=False)

@@ -191,7 +191,9 @@ def _heads_view(t: torch.Tensor, what: str):
     lead = t.shape[:-2]
     rows = math.prod(lead)
     if t.dim() == 3:
-        stride = t.stride(0)
+        stride = t.stride(0) if rows > 1 else h * d
+        if stride < h * d:   # an expanded tensor's 0 would be read as contiguous
+            raise ValueError(f"{what}: rows must not overlap")
     else:  # leading dims must collapse to one row stride
         stride = h * d
         if not t.is_contiguous():
@@ -342,6 +344,8 @@ def _attn_operand(t: torch.Tensor, shape, dtype, what: str, name: str):
     r, h, d = t.stride()
     if d != 1 and t.numel() > 0:
         raise ValueError(f"{what}: {name} must have unit stride on its last dim")
+    if (r == 0 and shape[0] > 1) or (h == 0 and shape[1] > 1):   # 0 would be read as contiguous
+        raise ValueError(f"{what}: {name} must not be expanded")
     return (r if shape[0] > 1 else 0, h if shape[1] > 1 else 0)
 
 
