@@ -77,6 +77,17 @@ def test_attention_refuses_aliases_and_workspaces(lib):
     assert bwd(lib, ws=ctypes.c_void_p(24)) == -1 and b"16-byte aligned" in lib.t2h_last_error()
 
 
+def test_gradients_that_alias_each_other(lib):
+    """Their blocks run side by side: one would overwrite the other's."""
+    R, S = ctypes.c_void_p(1 << 21), ctypes.c_void_p(1 << 22)
+    for args in (dict(dq=R, dk=R, dv=S), dict(dq=R, dk=S, dv=R), dict(dq=R, dk=S, dv=S)):
+        assert bwd(lib, **args) == -1 and b"alias each other" in lib.t2h_last_error()
+    kw = dict(q=ctypes.c_void_p(512), k=ctypes.c_void_p(1024), dq=ctypes.c_void_p(2048), dk=ctypes.c_void_p(4096))
+    for args in (dict(), dict(dqi=kw["dk"]), dict(dki=kw["dq"]), dict(dqi=kw["k"]), dict(dki=kw["q"]),
+                 dict(dq=P, dk=P, dqi=P, dki=P)):
+        assert qkb(lib, **{**kw, **args}) == -1 and b"must not alias" in lib.t2h_last_error()
+
+
 def test_expanded_tensors_are_refused(monkeypatch):
     """A stride of 0 means contiguous to the C ABI: it would read past an
     expanded tensor's end. A dimension of one has no stride that counts."""

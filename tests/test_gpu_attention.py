@@ -425,7 +425,7 @@ def test_rows_far_apart(dev, rows, d):
     assert torch.equal(out, again)
 
 
-def test_expanded_gradients_are_refused(dev):
+def test_expanded_gradients_and_aliases_are_refused(dev):
     from t2h import ops
 
     q, k, v, g = make(3, 20, 20, 2, 2, 64, F16, dev)
@@ -439,3 +439,8 @@ def test_expanded_gradients_are_refused(dev):
         ops.attention_backward(g[:, :, :1].expand(20, 2, 64), q, k, v, out, lse)
     with pytest.raises(ValueError, match="rows must not overlap"):
         ops.qk_rmsnorm_rope_backward(dq=g[:1].expand(20, 2, 64), use_rope=False)
+    dq = torch.empty_like(q)
+    with pytest.raises(Exception, match="alias each other"):
+        ops.attention_backward(g, q, k, v, out, lse, dq=dq, dk=dq)
+    with pytest.raises(Exception, match="must not alias"):
+        ops.qk_rmsnorm_rope_backward(dq=g, dk=g, use_rope=False, in_place=True)

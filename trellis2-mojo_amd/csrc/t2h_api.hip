@@ -484,6 +484,12 @@ int32_t t2h_qk_rmsnorm_rope_backward(const void* q_in, const void* k_in, const v
         return fail(T2H_EINVAL, "%s: needs a workspace of %lld bytes (16-byte aligned)", fn,
                     (long long)qk_bwd_bytes(rows, heads, head_dim, a.tensors));
     if (!sums) workspace = nullptr;
+    // q's and k's blocks run side by side
+    for (int i = 0; i < 2 && rows > 0 && a.tensors == 2; ++i) {
+        const QkBwdTensor &t = a.t[i], &o = a.t[1 - i];
+        if (t.dx == o.dx || t.dx == o.dy || (t.dx == o.x && o.gamma != nullptr))
+            return fail(T2H_EINVAL, "%s: q's and k's gradients must not alias", fn);
+    }
     if (rows == 0 && !sums) return ok();
     a.rows = rows;
     a.x_stride = in_stride;
@@ -661,6 +667,8 @@ int32_t t2h_attention_backward(const void* q, const void* k, const void* v, cons
     const int64_t need = attn_bwd_plan(a, workspace);
     if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need)
         return fail(T2H_EINVAL, "%s: needs a workspace of %lld bytes (16-byte aligned)", fn, (long long)need);
+    if ((q_rows > 0 && (dq == dk || dq == dv)) || (k_rows > 0 && dk == dv))
+        return fail(T2H_EINVAL, "%s: gradients must not alias each other", fn);
     a.dout = dout;
     a.dq = dq;
     a.dk = dk;
