@@ -111,10 +111,10 @@ def test_norm_bias_and_coords(dev, dtype, rows, h, d):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("source", ["none", "grid", "phases"])
 @pytest.mark.parametrize("d", [64, 128, 80])
-def test_one_tensor_position_sources_and_no_norm(dev, dtype, source, d):
+@pytest.mark.parametrize("rows,h", [(150, 4), (47, 9), (128, 3)])
+def test_one_tensor_position_sources_and_no_norm(dev, dtype, source, d, rows, h):
     from t2h import ops
 
-    rows, h = 150, 4
     (q, _, dq, _), (gq, _, bq, _) = tensors(d, rows, h, d, dtype, dev)
     f = freqs(d)
     kw, pos = dict(use_rope=False), None
@@ -142,10 +142,10 @@ def test_one_tensor_position_sources_and_no_norm(dev, dtype, source, d):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
-def test_packed_views_and_in_place(dev, dtype):
+@pytest.mark.parametrize("rows,h,d", [(211, 12, 128), (40, 13, 64)])
+def test_packed_views_and_in_place(dev, dtype, rows, h, d):
     from t2h import ops
 
-    rows, h, d = 211, 12, 128
     g = torch.Generator().manual_seed(0)
     qkv = torch.randn((rows, 3, h, d), generator=g).to(dtype).to(dev)
     dqkv = torch.randn((rows, 3, h, d), generator=g).to(dtype).to(dev)

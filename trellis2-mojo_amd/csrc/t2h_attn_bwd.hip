@@ -539,8 +539,8 @@ constexpr int kSplitRows = 1024;                   // streaming tokens that a pa
 // Few queries or few keys (kFine in all): P and dS keep twice the type's bits, as
 // two products. Such calls wait for memory, not for the matrix cores, and in their
 // results a few terms of a sum weigh most, whose rounding does not average out
-// (one query, 10,474 keys, f16: dk 3.4e-4 off in the 2-norm, 2.2e-4 so, of which
-// 2.1e-4 is its own rounding; 16 queries, 60,000 keys 323 -> 381 us).
+// (one query, 10,474 keys, f16: dk is 3.4e-4 off in the 2-norm, and so as little
+// as its own rounding, 2.2e-4; 16 queries, 60,000 keys 323 -> 381 us).
 struct Plan { bool small; int split; };
 Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads, bool fine) {
     const int64_t cu = device_cu_count(), per = (int64_t)nbatch * heads;

@@ -21,7 +21,9 @@
 namespace t2h {
 namespace {
 
-constexpr int kW = 4;   // waves per block
+constexpr int kW = 4;        // waves per block
+constexpr int kShortW = 16;  // ... of the form for few rows
+constexpr int kShort = 48;   // rows that it takes
 
 template <int LPH>
 __device__ __forceinline__ float head_sum(float v) {
@@ -55,34 +57,37 @@ template <typename T, int D, int NG, int LPH> struct RowPieces {
 };
 
 // Head layout as the forward's (HeadLanes): LPH lanes per head, NG groups of
-// 64 / LPH heads.
-template <typename T, int D, int NG>
-__global__ __launch_bounds__(kW * 64, sizeof(T) == 2 && NG < 4 ? 3 : 2) void qk_bwd_kernel(QkBwdArgs a, RopeSlots tab) {
+// 64 / LPH heads. SHORT (few rows): a block takes all rows of one group of heads
+// and writes the sums themselves, without a second launch.
+template <typename T, int D, int NG, int W, bool SHORT>
+__global__ __launch_bounds__(W * 64, SHORT ? 4 : sizeof(T) == 2 && NG < 4 ? 3 : 2) void qk_bwd_kernel(QkBwdArgs a, RopeSlots tab) {
     constexpr int LPH = (sizeof(T) == 2 && D == 64) ? 8 : 16;
     constexpr int HPI = 64 / LPH;
     using L = HeadLanes<T, D, LPH>;
     using Pieces = RowPieces<T, D, NG, LPH>;
     constexpr int E = L::E, P = L::P, HALF = D / 2;
     // gamma * scale and bias while rows are worked on, the waves' sums afterwards
-    __shared__ __attribute__((aligned(16))) float lds[kW][NG * HPI * D];
+    __shared__ __attribute__((aligned(16))) float lds[W][NG * HPI * D];
     const int lane = lane_id(), g = lane / LPH, m = lane % LPH;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int H = a.heads, HD = H * D;
     const int which = (int)(blockIdx.x % a.tensors);
     const QkBwdTensor& t = a.t[which];
-    const int64_t blk = blockIdx.x / a.tensors;
-    const T* __restrict__ x = static_cast<const T*>(t.x);
-    const T* __restrict__ dy = static_cast<const T*>(t.dy);
-    T* __restrict__ dx = static_cast<T*>(t.dx);
+    const int64_t blk = SHORT ? 0 : blockIdx.x / a.tensors;
+    // the block's heads: all, or HPI from head0 on
+    const int head0 = SHORT ? (int)(blockIdx.x / a.tensors) * HPI : 0, at0 = head0 * D;
+    const int H = SHORT ? (a.heads - head0 < HPI ? a.heads - head0 : HPI) : a.heads, HD = H * D;
+    const T* __restrict__ x = static_cast<const T*>(t.x) + at0;
+    const T* __restrict__ dy = static_cast<const T*>(t.dy) + at0;
+    T* __restrict__ dx = static_cast<T*>(t.dx) + at0;
     const bool norm = t.gamma != nullptr, biased = norm && t.bias != nullptr;
     const bool turn = a.use_rope && a.phases == nullptr;
     const PosSource src{a.coords, a.coord_cols, a.grid_res, a.pos_dim};
     const int my_slot = lane % HALF;
     const int my_axis = turn ? slot_axis(my_slot, a.freq_dim, a.pos_dim) : -1;
     const float my_freq = tab.freq[my_slot];
-    const int64_t step = a.blocks * kW;
+    const int64_t step = SHORT ? W : a.blocks * W;
 
-    int64_t r = blk * kW + wave;
+    int64_t r = blk * W + wave;
     Pieces xn, gn;
     int pos = 0;
     if (r < a.rows) {
@@ -91,9 +96,9 @@ __global__ __launch_bounds__(kW * 64, sizeof(T) == 2 && NG < 4 ? 3 : 2) void qk_
         if (norm) xn.load(x + r * a.x_stride, H, g, m);
     }
     if (norm)
-        for (int c = threadIdx.x; c < HD; c += kW * 64) {
-            lds[0][c] = t.gamma[c] * a.rms_scale;
-            if (biased) lds[1][c] = t.bias[c];
+        for (int c = threadIdx.x; c < HD; c += W * 64) {
+            lds[0][c] = t.gamma[at0 + c] * a.rms_scale;
+            if (biased) lds[1][c] = t.bias[at0 + c];
         }
     __syncthreads();
     float sg[NG][E], sb[NG][E];
@@ -168,7 +173,8 @@ __global__ __launch_bounds__(kW * 64, sizeof(T) == 2 && NG < 4 ? 3 : 2) void qk_
     float* part = a.part + ((int64_t)which * a.blocks + blk) * 2 * HD;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        if ((k == 0 ? t.dgamma : t.dbias) == nullptr) continue;
+        float* sum = k == 0 ? t.dgamma : t.dbias;
+        if (sum == nullptr) continue;
 #pragma unroll
         for (int i = 0; i < NG; ++i)
             if (HPI * i + g < H) {
@@ -176,11 +182,12 @@ __global__ __launch_bounds__(kW * 64, sizeof(T) == 2 && NG < 4 ? 3 : 2) void qk_
                 for (int e = 0; e < E; ++e) lds[wave][(HPI * i + g) * D + L::elem(m, e)] = k == 0 ? sg[i][e] : sb[i][e];
             }
         __syncthreads();
-        for (int c = threadIdx.x; c < HD; c += kW * 64) {
+        for (int c = threadIdx.x; c < HD; c += W * 64) {
             float s = lds[0][c];
 #pragma unroll
-            for (int w = 1; w < kW; ++w) s += lds[w][c];
-            part[k * HD + c] = s;
+            for (int w = 1; w < W; ++w) s += lds[w][c];
+            if constexpr (SHORT) sum[at0 + c] = k == 0 ? s * a.rms_scale : s;
+            else part[k * HD + c] = s;
         }
         __syncthreads();
     }
@@ -319,7 +326,7 @@ inline bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uint
 
 template <typename T, int D, int NG>
 void launch_fast(const QkBwdArgs& a, const RopeSlots& tab, hipStream_t s) {
-    hipLaunchKernelGGL((qk_bwd_kernel<T, D, NG>), dim3((unsigned)(a.blocks * a.tensors)), dim3(kW * 64), 0, s, a, tab);
+    hipLaunchKernelGGL((qk_bwd_kernel<T, D, NG, kW, false>), dim3((unsigned)(a.blocks * a.tensors)), dim3(kW * 64), 0, s, a, tab);
 }
 
 template <typename T>
@@ -335,6 +342,15 @@ hipError_t launch_typed(const QkBwdArgs& a, const RopeSlots& tab, hipStream_t s)
                aligned_to(a.t[i].gamma, 16) && aligned_to(a.t[i].bias, 16);
     if (a.rows == 0) {
         // nothing but the sums, of no partial rows
+    } else if (fast && a.rows <= kShort) {
+        // both tensors of 16 heads of 64 (bf16), replayed, against two launches:
+        // 1 row 6.5 -> 3.5 us, 37 rows 7.0 -> 6.4, 48 rows 6.9 -> 7.4 and 64 rows
+        // 7.0 -> 8.8; eagerly every call saves another 2.5 us of launching
+        const int hpi = sizeof(T) == 2 && a.head_dim == 64 ? 8 : 4;
+        const dim3 grid((unsigned)((a.heads + hpi - 1) / hpi * a.tensors));
+        if (a.head_dim == 128) hipLaunchKernelGGL((qk_bwd_kernel<T, 128, 1, kShortW, true>), grid, dim3(kShortW * 64), 0, s, a, tab);
+        else hipLaunchKernelGGL((qk_bwd_kernel<T, 64, 1, kShortW, true>), grid, dim3(kShortW * 64), 0, s, a, tab);
+        return hipGetLastError();
     } else if (!fast) {
         const int64_t units = a.blocks * a.heads;
         hipLaunchKernelGGL((qk_bwd_generic<T>), dim3((unsigned)((units + kW - 1) / kW * a.tensors)), dim3(kW * 64), 0, s, a, tab);
