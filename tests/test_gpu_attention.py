@@ -444,3 +444,18 @@ def test_expanded_gradients_and_aliases_are_refused(dev):
         ops.attention_backward(g, q, k, v, out, lse, dq=dq, dk=dq)
     with pytest.raises(Exception, match="must not alias"):
         ops.qk_rmsnorm_rope_backward(dq=g, dk=g, use_rope=False, in_place=True)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,krows", [(0, 1000), (1000, 0), (0, 20)])
+def test_segments_of_a_tensor_without_rows(dev, dtype, rows, krows):
+    """Offsets over an empty side, the other long enough to be split."""
+    from t2h import ops
+
+    q, k, v, g = make(21, rows, krows, 2, 2, 64, dtype, dev)
+    seg = dict(nbatch=2, q_offsets=offs([rows // 2] * 2, dev)[1], k_offsets=offs([krows // 2] * 2, dev)[1])
+    out, lse = ops.attention(q, k, v, need_lse=True, **seg)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    for x in ops.attention_backward(g, q, k, v, out, lse, **seg):
+        assert (x == 0).all()
+    torch.cuda.synchronize()

@@ -587,7 +587,7 @@ hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
     else a.q_small ? launch_forms<T, D, 2, 1>(a, s) : launch_forms<T, D, 2, 2>(a, s);
     SumArgs m{};
     m.nbatch = f.nbatch;
-    if (a.kv_split > 1 && a.kv_blocks > 0) {
+    if (a.kv_split > 1 && f.k_rows > 0) {
         m.part[0] = a.part_kv;
         m.part[1] = a.part_kv + a.kv_split * f.k_rows * a.kv_heads * D;
         m.out[0] = a.dk;
@@ -602,7 +602,7 @@ hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
         m.nsplit = a.kv_split;
         launch_sums<T, D>(m, 2, s);
     }
-    if (a.q_split > 1 && a.q_blocks > 0) {
+    if (a.q_split > 1 && f.q_rows > 0) {
         m.part[0] = a.part_q;
         m.out[0] = a.dq;
         m.row_stride[0] = a.dq_row;
