@@ -2,6 +2,23 @@
 //
 //   s_ij = scale * sum_d q_id k_jd       lse_i = log sum_j exp(s_ij)
 //   out_i = sum_j exp(s_ij - lse_i) v_j
+//
+// One pass over the keys with each row's running sum of exponentials and a
+// reference m near its running maximum: out = sum_j exp(s_ij - m) v_j / sum_j
+// exp(s_ij - m) for any m. m moves only when a tile's maximum is more than 2^8
+// above it, so most tiles rescale nothing, and the exponentials stay below 2^8 (f16
+// holds 2^16).
+//
+// 4 D operations a score on the matrix cores, one exponential: from some hundred
+// queries on the products bound it. There the tiles and their order serve to keep
+// the matrix cores fed: the next tile's scores run under this tile's exponentials,
+// K and V come to LDS one tile ahead, their fragments serve 32 queries, and two
+// blocks a CU cover each other's barriers. Measured (f16, 12 heads of 128): two
+// segments of 39,804 tokens in all 4.33 ms, 1,130 TFLOP/s, where the library's
+// largest products reach 1,300 on the same card; the matrix cores are busy 57 % of
+// the cycles, LDS has no conflicts, and the clock falls to 1.7-2.0 GHz of 2.4: power
+// bounds both. 4,096 tokens (bf16) 110 us, 935 TFLOP/s: 384 blocks on 512 places.
+// Few queries read K and V once from memory: 100,000 keys 118 us, 5.2 TB/s.
 #include <type_traits>
 
 #include "t2h_attn_core.h"
@@ -276,7 +293,10 @@ __global__ __launch_bounds__(NW * KG * 64, 2) void attn_kernel(AttnArgs a) {
 
 // Join of the splits: out = sum_s exp2(lse_s - lse) out_s. A wave takes STRANDS
 // splits at a time of 4 / STRANDS (row, head)s, 16 lanes each, D / 16 elements a
-// lane; WAVES waves share a (row, head)'s splits and meet in LDS.
+// lane; WAVES waves share a (row, head)'s splits and meet in LDS. Up to 8 splits
+// (many rows) one strand each; more would be a chain of as many loads, and go to 16
+// strands (whole calls: 1,000 queries in 4 splits one strand 17.0 us, 16 20.3; one
+// query in 16 splits 13.2 and 9.6, in 64 42 and 24).
 template <typename T, int D, int STRANDS, int WAVES>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     constexpr int E = D / 16, kUnits = 16 / (STRANDS * WAVES);
@@ -356,6 +376,15 @@ struct Small { static constexpr int nw = 4, nt = 1, kt = 64; template <int D> st
 struct Few { static constexpr int nw = 1, nt = 1, kt = 32; template <int D> static constexpr int kg = D == 64 ? 8 : 4; };
 enum Form { kLarge, kSmall, kFew };
 
+// Few: segments of no more queries than its tile, whose other forms' waves would
+// be idle (1 query, 16 heads of 64, 512 keys: 6.0 us, small in parts 7.1; 100,000
+// keys, 12 heads of 128: 118 and 120); 17 to 48 queries leave it two and three
+// tiles that read the keys again (32 queries, 10,474 keys: 21.0, small 18.0).
+// Large: where its blocks fill 1.5 places a CU; below, the small form's twice as
+// many blocks do better (2,368 queries, 1,029 keys, 16 heads of 64: small 23.6 us,
+// large 26.9; 8,192 queries, 12 heads of 128: 73 and 62), and for segments within
+// its tile (64 of 37 tokens: 6.9 and 9.5).
+
 Form form_of(const AttnArgs& a) {
     const int64_t rows = (a.q_rows + a.nbatch - 1) / a.nbatch, cu = device_cu_count();
     if (rows <= 16) return kFew;
@@ -388,14 +417,21 @@ hipError_t launch_d(AttnArgs a, hipStream_t s) {
 
 }  // namespace
 
+// Parts of the keys: as many as idle CUs take, of 128 keys at least. One query,
+// replayed, in one part / in parts: 16 heads of 64, 512 keys 6.0 / 7.3 us, 1,029
+// keys 8.3 / 8.0 (and a second launch's 2.5 us where the host waits for it); 12
+// heads of 128, 1,500 keys 14.7 / 9, 2,058 keys 20 / 9.5, 10,474 keys 92 / 17.7. Parts of
+// 1,024 keys at least: 14.6 and 20.3; two blocks a CU: 9.5 and 20.9. 48 queries,
+// 1,029 keys 11.2 / 8.3; 300 queries, 10,474 keys 123 / 39.
 int attn_splits(const AttnArgs& a) {
+    // few queries: keys that a block takes in six turns stay in one launch
+    const int64_t one_part = 6 * Few::kt * (a.head_dim == 64 ? Few::kg<64> : Few::kg<128>);
     const int64_t rows = (a.q_rows + a.nbatch - 1) / a.nbatch, keys = a.k_rows / a.nbatch;
     const Form f = form_of(a);
-    if (f != kSmall && f != kFew) return 1;
+    if (f == kLarge || (f == kFew && keys <= one_part)) return 1;
     const int64_t tiles = (rows + (f == kFew ? 15 : 63)) / (f == kFew ? 16 : 64) * a.nbatch * a.heads;
     int64_t n = device_cu_count() / (tiles > 0 ? tiles : 1);
-    const int64_t least = f == kFew ? 1024 : 128;
-    if (n > keys / least) n = keys / least;
+    if (n > keys / 128) n = keys / 128;
     if (n > 64) n = 64;
     return n < 1 ? 1 : (int)n;
 }

@@ -162,7 +162,8 @@ def scaled_dot_product_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     if k.shape[0] != n or k.shape[3] != d:
         raise ValueError("scaled_dot_product_attention: q/k shape mismatch")
     flat = lambda t: t.reshape(-1, t.shape[2], d)
-    return ops.attention(flat(q), flat(k), flat(v), nbatch=n, k_lens=k_lens).reshape(q.shape)
+    return ops.attention(flat(q), flat(k), flat(v), nbatch=max(n, 1),
+                         k_lens=k_lens if n > 0 else None).reshape(q.shape)
 
 
 def _gate(x: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
