@@ -47,7 +47,7 @@ struct AttnBwdArgs {
     int32_t kv_heads;
     // set by attn_bwd_plan: forms, parts, and the workspace's pieces
     int32_t kv_split, q_split;
-    bool kv_small, q_small, fine;
+    bool kv_small, q_small, fine, q_first;
     float* delta;            // [heads, q_rows]
     float* lse2;             // [heads, q_rows] log2, less the rounding shift of P
     float* g_most;           // [heads, prep_q_tiles] f16: largest squared row length of dout in each tile

@@ -485,42 +485,52 @@ __device__ __forceinline__ void dkv_block(const AttnBwdArgs& a, uint8_t* lds, in
     }
 }
 
-// Blocks for dk and dv first: they take longer.
+// The side with the longer blocks comes first (q_first), so that the others fill
+// the GPU as those end.
 template <typename T, int D, int KV, int Q>
 __global__ __launch_bounds__(256, 2) void attn_bwd_kernel(AttnBwdArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kQT * D * 2 + 4 * kQT * 4];
-    const int64_t p = block_linear();
-    if (p < a.kv_blocks) dkv_block<T, D, 4, KV>(a, lds, (int)p);
-    else if (p - a.kv_blocks < a.q_blocks) dq_block<T, D, 4, Q>(a, lds, (int)(p - a.kv_blocks));
+    int64_t p = block_linear();
+    if (p >= (int64_t)a.kv_blocks + a.q_blocks) return;
+    const int first = a.q_first ? a.q_blocks : a.kv_blocks;
+    const bool q = (p < first) == a.q_first;
+    if (p >= first) p -= first;
+    if (q) dq_block<T, D, 4, Q>(a, lds, (int)p);
+    else dkv_block<T, D, 4, KV>(a, lds, (int)p);
 }
 
-// Sum of the parts [nsplit, rows, heads, D] in order; blockIdx.z: part set
-// (dk, dv) and output.
-struct SumArgs {
-    const float* part[2];
-    void* out[2];
-    int64_t row_stride[2], head_stride[2];
+// Sums of the parts [nsplit, rows, heads, D] in order; blockIdx.z: which of dk,
+// dv and dq.
+struct SumSet {
+    const float* part;
+    void* out;
+    int64_t row_stride, head_stride, rows;
     const int64_t* offsets;   // rows outside the segments are left alone
-    int64_t rows;
-    int32_t heads, nsplit, nbatch;
+    int32_t heads, nsplit;
+};
+struct SumArgs {
+    SumSet set[3];
+    int32_t nbatch;
 };
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_sum_kernel(SumArgs a) {
+__global__ __launch_bounds__(256) void attn_sum_kernel(SumArgs args) {
     constexpr int E = D / 16;
+    const SumSet& a = args.set[blockIdx.z];
     const int64_t u = block_linear() * 16 + threadIdx.x / 16;
     if (u >= a.rows * a.heads) return;
     const int64_t row = u / a.heads;
     const int head = (int)(u - row * a.heads);
-    if (a.offsets != nullptr && (row < a.offsets[0] || row >= a.offsets[a.nbatch])) return;
-    const int m = threadIdx.x & 15, w = blockIdx.z;
+    if (a.offsets != nullptr && (row < a.offsets[0] || row >= a.offsets[args.nbatch])) return;
+    const int m = threadIdx.x & 15;
     float acc[E] = {};
+#pragma unroll 4
     for (int s = 0; s < a.nsplit; ++s) {
         float v[E];
-        load_params<E>(a.part[w] + (((int64_t)s * a.rows + row) * a.heads + head) * D + m * E, v);
+        load_params<E>(a.part + (((int64_t)s * a.rows + row) * a.heads + head) * D + m * E, v);
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += v[e];
     }
-    store_elems<T, E>(static_cast<T*>(a.out[w]) + row * a.row_stride[w] + head * a.head_stride[w] + m * E, acc);
+    store_elems<T, E>(static_cast<T*>(a.out) + row * a.row_stride + head * a.head_stride + m * E, acc);
 }
 
 // Four waves a block, two blocks a CU; a wave keeps two 16-token tiles (the large
@@ -535,13 +545,20 @@ constexpr int kSplitRows = 1024;                   // streaming tokens that a pa
 // 19,902 queries in 2 parts 677 us, 3: 692, 6: 718); where the parts would be too
 // short for 1.5 blocks a CU (300 queries, 3,000 keys: large 57.6 us, small 51.5),
 // and for segments no longer than its tile (64 of 37 tokens, 16 heads of 64, each
-// side's blocks alone: 12.2 and 12.5 us, small 8.5 and 9.9), the small form.
+// side's blocks alone: 12.2 and 12.5 us, small 8.5 and 9.9), the small form, in
+// parts of 128 streaming tokens at least, from 512 on (64 queries, 1,029 keys, 16
+// heads of 64: in parts of 128 15.7 us, 256 16.0, 512 21; 300 queries and keys: 2
+// parts 16.6, one 12.1). Two blocks a CU there: 24 us for 20.
+// Where both sides' small blocks are fewer than the CUs, the parts are such that
+// all blocks of both take one CU each for about as long, 256 tokens at least (512
+// queries and keys, 16 heads of 64: each side by itself 2 parts 23.6 us, one 17.1;
+// 4 heads of 128, 1,024: 4 parts 36.6, 2 38.7; 512 and 2,000, 2 heads 32.0, 29.0).
 // Few queries or few keys (kFine in all): P and dS keep twice the type's bits, as
 // two products. Such calls wait for memory, not for the matrix cores, and in their
 // results a few terms of a sum weigh most, whose rounding does not average out
 // (one query, 10,474 keys, f16: dk is 3.4e-4 off in the 2-norm, and so as little
 // as its own rounding, 2.2e-4; 16 queries, 60,000 keys 323 -> 381 us).
-struct Plan { bool small; int split; };
+struct Plan { bool small; int split; int64_t blocks; };   // blocks: of the small form, unsplit
 Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads, bool fine) {
     const int64_t cu = device_cu_count(), per = (int64_t)nbatch * heads;
     const int64_t large = ((int64_t)kept.share + kRowsLarge - 1) / kRowsLarge * per;
@@ -551,21 +568,28 @@ Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads
     p.small = large * most * 2 < 3 * cu || kept.share <= kRowsSmall || fine;
     int64_t n = 1;
     if (p.small) {
-        n = cu / (small > 0 ? small : 1);
+        n = stream < 512 ? 1 : cu / (small > 0 ? small : 1);
         if (n > stream / 128) n = stream / 128;
     } else if (large * 2 < 3 * cu) {
         n = 2 * cu / large;
         if (n > most) n = most;
     }
     p.split = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    p.blocks = small;
     return p;
 }
-
-template <typename T, int D>
-void launch_sums(const SumArgs& m, int sets, hipStream_t s) {
-    dim3 grid = grid_1d((m.rows * m.heads + 15) / 16);
-    grid.z = sets;
-    hipLaunchKernelGGL((attn_sum_kernel<T, D>), grid, dim3(256), 0, s, m);
+// Parts for both sides' small blocks at once; a block of dk, dv does 4 products
+// a streaming token, one of dq 3.
+void share_cus(Plan& q, int64_t keys, Plan& kv, int64_t queries) {
+    const int64_t cu = device_cu_count();
+    if (!q.small || !kv.small || q.blocks + kv.blocks > cu) return;
+    const int64_t each = (q.blocks * keys * 3 + kv.blocks * queries * 4) / (cu * 4), len = each > 256 ? each : 256;
+    const auto parts = [len](int64_t stream) {
+        const int64_t n = (stream + len / 2) / len;
+        return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    };
+    q.split = parts(keys);
+    kv.split = parts(queries);
 }
 
 template <typename T, int D, int KV, int Q>
@@ -587,31 +611,24 @@ hipError_t launch_d(AttnBwdArgs a, hipStream_t s) {
     else a.q_small ? launch_forms<T, D, 2, 1>(a, s) : launch_forms<T, D, 2, 2>(a, s);
     SumArgs m{};
     m.nbatch = f.nbatch;
+    int sets = 0;
+    int64_t units = 0;
+    const auto add = [&](const float* part, void* out, int64_t row, int64_t head, int64_t rows, const AttnSide& side,
+                         int32_t heads, int32_t nsplit) {
+        m.set[sets++] = SumSet{part, out, row, head, rows, side.offsets, heads, nsplit};
+        if (rows * heads > units) units = rows * heads;
+    };
     if (a.kv_split > 1 && f.k_rows > 0) {
-        m.part[0] = a.part_kv;
-        m.part[1] = a.part_kv + a.kv_split * f.k_rows * a.kv_heads * D;
-        m.out[0] = a.dk;
-        m.out[1] = a.dv;
-        m.row_stride[0] = a.dk_row;
-        m.row_stride[1] = a.dv_row;
-        m.head_stride[0] = a.dk_head;
-        m.head_stride[1] = a.dv_head;
-        m.offsets = f.ks.offsets;
-        m.rows = f.k_rows;
-        m.heads = a.kv_heads;
-        m.nsplit = a.kv_split;
-        launch_sums<T, D>(m, 2, s);
+        const float* pv = a.part_kv + a.kv_split * f.k_rows * a.kv_heads * D;
+        add(a.part_kv, a.dk, a.dk_row, a.dk_head, f.k_rows, f.ks, a.kv_heads, a.kv_split);
+        add(pv, a.dv, a.dv_row, a.dv_head, f.k_rows, f.ks, a.kv_heads, a.kv_split);
     }
-    if (a.q_split > 1 && f.q_rows > 0) {
-        m.part[0] = a.part_q;
-        m.out[0] = a.dq;
-        m.row_stride[0] = a.dq_row;
-        m.head_stride[0] = a.dq_head;
-        m.offsets = f.qs.offsets;
-        m.rows = f.q_rows;
-        m.heads = f.heads;
-        m.nsplit = a.q_split;
-        launch_sums<T, D>(m, 1, s);
+    if (a.q_split > 1 && f.q_rows > 0)
+        add(a.part_q, a.dq, a.dq_row, a.dq_head, f.q_rows, f.qs, f.heads, a.q_split);
+    if (sets > 0) {
+        dim3 grid = grid_1d((units + 15) / 16);
+        grid.z = sets;
+        hipLaunchKernelGGL((attn_sum_kernel<T, D>), grid, dim3(256), 0, s, m);
     }
     return hipGetLastError();
 }
@@ -628,13 +645,18 @@ int64_t attn_bwd_plan(AttnBwdArgs& a, void* workspace) {
     a.prep_k_tiles = (int32_t)tile_count(f.ks, f.nbatch, kPrepRows);
     a.prep_blocks = a.prep_q_tiles * f.heads + (f.dtype == T2H_F16 ? a.prep_k_tiles * a.kv_heads : 0);
     const bool fine = f.q_rows <= kFine || f.k_rows <= kFine;
-    const Plan q = plan_of(f.qs, f.ks.share, f.nbatch, f.heads, fine);
-    const Plan kv = plan_of(f.ks, (int64_t)f.qs.share * f.group, f.nbatch, a.kv_heads, fine);
+    const int64_t queries = (int64_t)f.qs.share * f.group;    // that a key's block reads
+    Plan q = plan_of(f.qs, f.ks.share, f.nbatch, f.heads, fine);
+    Plan kv = plan_of(f.ks, queries, f.nbatch, a.kv_heads, fine);
+    share_cus(q, f.ks.share, kv, queries);
     a.q_small = q.small;
     a.q_split = q.split;
     a.kv_small = kv.small;
     a.fine = fine;
     a.kv_split = kv.split;
+    // a block's products: streaming tokens x kept tiles a wave x 4 or 3
+    a.q_first = (int64_t)f.ks.share / q.split * (q.small ? 1 : 2) * 3 >
+                queries / kv.split * (kv.small ? 1 : 2) * 4;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     int64_t at = 0;
     const auto take = [&](int64_t floats) {
