@@ -215,7 +215,8 @@ int32_t t2h_attn_pack(const void* q, const void* k, const void* v,
  * q, out [q_rows, heads, head_dim], k, v [k_rows, kv_heads, head_dim], f16 or
  * bf16, head_dim 64 or 128; heads a multiple of kv_heads (query head h reads
  * key/value head h / (heads / kv_heads)). Sums and softmax in f32; the
- * exponentials are rounded to dtype for the product with v.
+ * exponentials are rounded to dtype for the product with v (up to 16 queries a
+ * segment: to twice its bits).
  * strides_host: (row, head) strides in elements of q, k, v, out (8 values; 0 =
  * contiguous), so that the operands can be views of a packed qkv [rows, 3, H,
  * D] (row 3HD, head D) or the head-major outputs of t2h_attn_pack /
@@ -225,7 +226,7 @@ int32_t t2h_attn_pack(const void* q, const void* k, const void* v,
  * [nbatch + 1]) or equal shares where a side's offsets are NULL. k_lens (int64
  * device [nbatch] or NULL): only that many keys at the start of a segment
  * count; what lies in the others is not used, whatever it is. A row without
- * keys gets out 0 and lse -inf. Rows outside the segments are not written.
+ * keys, or whose scores are all -inf, gets out 0 and lse -inf. Rows outside the segments are not written.
  * lse [heads, q_rows] f32 or NULL. out must not overlap the inputs.
  * workspace: t2h_attention_workspace() bytes (16-byte aligned, any contents)
  * let calls of few rows split their keys over the GPU; with less, or NULL,
@@ -249,7 +250,8 @@ int32_t t2h_attention(const void* q, const void* k, const void* v, void* out,
  *   dv_j = sum_i P_ij dout_i, dq_i = scale sum_j dS_ij k_j,
  *   dk_j = scale sum_i dS_ij q_i,
  * with dk and dv summed over the query heads of a key/value head. P and dS are
- * rounded to dtype for the products, sums are f32. Shapes and segments as
+ * rounded to dtype for the products (with at most 64 queries or keys: to twice
+ * its bits), sums are f32. Shapes and segments as
  * t2h_attention; strides_host: 16 values, of q, k, v, out, dout, dq, dk, dv.
  * Keys that do not count get dk = dv = 0, rows without keys dq = 0; rows
  * outside the segments are not written. The gradients must not overlap the
@@ -278,8 +280,8 @@ int32_t t2h_attention_backward(const void* q, const void* k, const void* v,
  *   dgamma = sqrt(head_dim) sum_rows g * xh, dbias = sum_rows din.
  * q_in / k_in: the forward's inputs (row stride in_stride; read only for a
  * norm), dq_out / dk_out the gradients of its outputs (dout_stride), dq_in /
- * dk_in those of its inputs (din_stride; in place on dq_out / dk_out with
- * equal strides). Either of q and k may be NULL throughout. Parameters and
+ * dk_in those of its inputs (din_stride; each in place on its own dq_out /
+ * dk_out with equal strides, else apart from all the others). Either of q and k may be NULL throughout. Parameters and
  * positions as in t2h_qk_rmsnorm_rope; gamma_q without gamma_k is allowed.
  * dgamma_*, dbias_* [heads, head_dim] f32, overwritten, or NULL; any of them
  * needs a workspace of t2h_qk_rmsnorm_rope_backward_workspace() bytes
