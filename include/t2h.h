@@ -226,7 +226,8 @@ int32_t t2h_attn_pack(const void* q, const void* k, const void* v,
  * [nbatch + 1]) or equal shares where a side's offsets are NULL. k_lens (int64
  * device [nbatch] or NULL): only that many keys at the start of a segment
  * count; what lies in the others is not used, whatever it is. A row without
- * keys, or whose scores are all -inf, gets out 0 and lse -inf. Rows outside the segments are not written.
+ * keys, or whose scores are all -inf, gets out 0 and lse -inf. Rows outside the
+ * segments are not written.
  * lse [heads, q_rows] f32 or NULL. out must not overlap the inputs.
  * workspace: t2h_attention_workspace() bytes (16-byte aligned, any contents)
  * let calls of few rows split their keys over the GPU; with less, or NULL,
@@ -281,8 +282,9 @@ int32_t t2h_attention_backward(const void* q, const void* k, const void* v,
  * q_in / k_in: the forward's inputs (row stride in_stride; read only for a
  * norm), dq_out / dk_out the gradients of its outputs (dout_stride), dq_in /
  * dk_in those of its inputs (din_stride; each in place on its own dq_out /
- * dk_out with equal strides, else apart from all the others). Either of q and k may be NULL throughout. Parameters and
- * positions as in t2h_qk_rmsnorm_rope; gamma_q without gamma_k is allowed.
+ * dk_out with equal strides, else apart from all the others). Either of q and k
+ * may be NULL throughout. Parameters and positions as in t2h_qk_rmsnorm_rope;
+ * gamma_q without gamma_k is allowed.
  * dgamma_*, dbias_* [heads, head_dim] f32, overwritten, or NULL; any of them
  * needs a workspace of t2h_qk_rmsnorm_rope_backward_workspace() bytes
  * (tensors: how many of q and k are given). The sums are f32, in a fixed

@@ -185,13 +185,13 @@ def _heads_view(t: torch.Tensor, what: str):
     _dev(t, what)
     if t.dim() < 3:
         raise ValueError(f"{what}: expected [..., H, D]")
-    h, d = t.shape[-2], t.shape[-1]
-    if t.stride(-1) != 1 or t.stride(-2) != d:
+    shape, st = t.shape, t.stride()
+    h, d = shape[-2], shape[-1]
+    if st[-1] != 1 or st[-2] != d:
         raise ValueError(f"{what}: heads must be contiguous [H, D]")
-    lead = t.shape[:-2]
-    rows = math.prod(lead)
-    if t.dim() == 3:
-        stride = t.stride(0) if rows > 1 else h * d
+    rows = shape[0] if len(shape) == 3 else math.prod(shape[:-2])
+    if len(shape) == 3:
+        stride = st[0] if rows > 1 else h * d
         if stride < h * d:   # an expanded tensor's 0 would be read as contiguous
             raise ValueError(f"{what}: rows must not overlap")
     else:  # leading dims must collapse to one row stride
@@ -336,6 +336,11 @@ def _same_device(ref: torch.Tensor, tensors, what: str) -> None:
             raise ValueError(f"{what}: tensors are on different devices")
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _attn_operand(t: torch.Tensor, shape, dtype, what: str, name: str):
     """[rows, H, D] with unit stride on D -> (row stride, head stride) in
     elements; 0 for a dimension of one, which has no stride of its own."""
@@ -410,7 +415,7 @@ def attention(q, k, v, scale: Optional[float] = None, q_offsets=None, k_offsets=
     rows, h, d = qs
     _attn_segments(what, nbatch, q_offsets, k_offsets, k_lens)
     if out is None:
-        out = torch.empty(qs, dtype=qd, device=q.device)
+        out = _like(q)
     strides = array.array("q", (*_attn_operand(q, qs, qd, what, "q"), *_attn_operand(k, ks, qd, what, "k"),
                                 *_attn_operand(v, ks, qd, what, "v"), *_attn_operand(out, qs, qd, what, "out")))
     lse = torch.empty((h, rows), dtype=torch.float32, device=q.device) if need_lse else None
@@ -438,10 +443,9 @@ def attention_backward(dout, q, k, v, out, lse, scale: Optional[float] = None, q
     _attn_segments(what, nbatch, q_offsets, k_offsets, k_lens)
     if lse.dtype != torch.float32 or lse.shape != (h, rows) or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be contiguous float32 [{h}, {rows}]")
-    mk = lambda shape: torch.empty(shape, dtype=qd, device=q.device)
-    dq = mk(qs) if dq is None else dq
-    dk = mk(ks) if dk is None else dk
-    dv = mk(ks) if dv is None else dv
+    dq = _like(q) if dq is None else dq
+    dk = _like(k) if dk is None else dk
+    dv = _like(v) if dv is None else dv
     strides = array.array("q", (*_attn_operand(q, qs, qd, what, "q"), *_attn_operand(k, ks, qd, what, "k"),
                                 *_attn_operand(v, ks, qd, what, "v"), *_attn_operand(out, qs, qd, what, "out"),
                                 *_attn_operand(dout, qs, qd, what, "dout"), *_attn_operand(dq, qs, qd, what, "dq"),
@@ -490,11 +494,11 @@ def qk_rmsnorm_rope_backward(dq=None, dk=None, q=None, k=None, gamma_q=None, gam
     if in_place:
         dqi, dki, din_stride = dq, dk, dy_stride
     else:
-        dqi, dki = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (dq, dk))
+        dqi, dki = None if dq is None else _like(dq), None if dk is None else _like(dk)
         din_stride = h * d
-    has = [t is not None and g is not None for t, g in ((gamma_q, dq), (gamma_k, dk), (bias_q, dq), (bias_k, dk))]
-    sums = iter(torch.empty((sum(has), h, d), dtype=torch.float32, device=ref.device).unbind(0) if any(has) else ())
-    dgq, dgk, dbq, dbk = (next(sums) if x else None for x in has)
+    mk = lambda t, g: None if t is None or g is None else (
+        torch.empty_like(t) if t.shape == (h, d) else t.new_empty((h, d)))
+    dgq, dgk, dbq, dbk = mk(gamma_q, dq), mk(gamma_k, dk), mk(bias_q, dq), mk(bias_k, dk)
     hold, fp, fd = _host_freqs(freqs if freqs is not None else [])
     ph_rows = 0
     if phases is not None:
@@ -507,7 +511,7 @@ def qk_rmsnorm_rope_backward(dq=None, dk=None, q=None, k=None, gamma_q=None, gam
             raise ValueError(f"{what}: coords must be contiguous int32 [rows, 1+pos_dim]")
         cc = coords.shape[1]
     ws = workspace
-    if any(has):
+    if dgq is not None or dgk is not None or dbq is not None or dbk is not None:
         need = _attn_bytes("t2h_qk_rmsnorm_rope_backward_workspace", rows, h, d, (dq is not None) + (dk is not None))
         ws = _attn_workspace(ws, max(need, 16), ref.device, what)
     p = _ptr
