@@ -164,3 +164,21 @@ def test_python_refuses_host_tensors():
         ops.qk_rmsnorm_rope_backward()
     with pytest.raises(ValueError):
         ops.attention_workspace(1, 1, 3, 2, 64)
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    """The launch goes to the current device's stream."""
+    class OnDevice:
+        def __init__(self, i):
+            self.i = i
+
+        def get_device(self):
+            return self.i
+
+    monkeypatch.setattr(ops, "_dev", lambda *a: None)
+    monkeypatch.setattr(ops, "_current", lambda: 0)
+    ops._same_device(OnDevice(0), (OnDevice(0), None), "f")
+    with pytest.raises(ValueError, match="f: tensors must be on the current device"):
+        ops._same_device(OnDevice(1), (OnDevice(1),), "f")
+    with pytest.raises(ValueError, match="f: tensors are on different devices"):
+        ops._same_device(OnDevice(0), (None, OnDevice(1)), "f")

@@ -459,3 +459,16 @@ def test_segments_of_a_tensor_without_rows(dev, dtype, rows, krows):
     for x in ops.attention_backward(g, q, k, v, out, lse, **seg):
         assert (x == 0).all()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype,rows,krows,h,kvh,d", [
+    (F16, 512, 512, 4, 4, 64), (BF16, 512, 512, 4, 2, 128),      # both sides in parts
+    (F16, 64, 1029, 2, 2, 64), (BF16, 1029, 64, 2, 2, 128),      # one side in parts, either side's blocks first
+    (F16, 2000, 512, 2, 1, 128), (BF16, 300, 3000, 12, 12, 128), (F16, 3000, 300, 12, 4, 64)])
+def test_backward_forms_and_parts(dev, dtype, rows, krows, h, kvh, d):
+    q, k, v, g = make(31, rows, krows, h, kvh, d, dtype, dev)
+    run_both(q, k, v, g, d ** -0.5, dev)
+    third = rows // 3
+    _, qo = offs([third, 0, rows - third - 7], dev)              # and ragged, with uncovered rows
+    _, ko = offs([krows - 9, 4, 5], dev)
+    run_both(q, k, v, g, d ** -0.5, dev, nbatch=3, q_offsets=qo, k_offsets=ko)
