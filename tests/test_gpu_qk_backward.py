@@ -249,3 +249,28 @@ def test_no_rows(dev):
     gq = torch.ones((2, 64), device=dev)
     r = ops.qk_rmsnorm_rope_backward(dq=z, q=z, gamma_q=gq, bias_q=gq, use_rope=False)
     assert r[0].shape == z.shape and (r[2] == 0).all() and (r[4] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,h,d", [(F16, 12, 128), (BF16, 16, 64), (F32, 5, 128)])
+def test_tensors_beyond_the_cache_against_pieces(dev, dtype, h, d):
+    """Large tensors are read by another policy: dx is the pieces' bit for bit.
+    A term g * xh of dgamma carries at most d + 8 roundings (the squares' sum, its
+    root, three products), a sum less than 200 additions one behind the other in
+    either form: 2 * (d + 208) 2^-24 of the terms' magnitudes."""
+    from t2h import ops
+
+    rows = (450 << 20) // (6 * h * d * torch.finfo(dtype).bits // 8)
+    g = torch.Generator(device=dev).manual_seed(4)
+    q, k, dq, dk = (torch.randn((rows, h, d), generator=g, device=dev).to(dtype) for _ in range(4))
+    gm = torch.randn((h, d), generator=g, device=dev) * 0.1 + 1
+    kw = dict(gamma_q=gm, gamma_k=gm, use_rope=False)
+    got = ops.qk_rmsnorm_rope_backward(dq=dq, dk=dk, q=q, k=k, **kw)
+    sums = [0.0, 0.0]
+    for at in range(0, rows, 7000):
+        s = slice(at, at + 7000)
+        want = ops.qk_rmsnorm_rope_backward(dq=dq[s], dk=dk[s], q=q[s], k=k[s], **kw)
+        assert torch.equal(got[0][s], want[0]) and torch.equal(got[1][s], want[1])
+        sums = [a + b.double() for a, b in zip(sums, want[2:4])]
+    for x, dy, total, want in ((q, dq, got[2], sums[0]), (k, dk, got[3], sums[1])):
+        terms = (dy.double() * torch.nn.functional.normalize(x.double(), dim=-1)).abs().sum(0) * d ** 0.5
+        assert ((total.double() - want).abs() <= 2 * (d + 208) * 2.0 ** -24 * terms).all()

@@ -39,7 +39,7 @@ __device__ __forceinline__ float head_sum(float v) {
 
 // One row's pieces of a wave, as loaded: the next row's are in flight while this
 // one is worked on.
-template <typename T, int D, int NG, int LPH> struct RowPieces {
+template <typename T, int D, int NG, int LPH, bool CACHED> struct RowPieces {
     using L = HeadLanes<T, D, LPH>;
     static constexpr int HPI = 64 / LPH;
     static constexpr int kWords = L::VE * (int)sizeof(T) / 4;   // 4, or 2 (f32 of head_dim 64 has 4 too)
@@ -50,8 +50,10 @@ template <typename T, int D, int NG, int LPH> struct RowPieces {
         for (int i = 0; i < NG; ++i) {
             const int hh = HPI * i + g < H ? HPI * i + g : H - 1;
 #pragma unroll
-            for (int j = 0; j < L::NC; ++j)
-                w[i][j] = __builtin_nontemporal_load(reinterpret_cast<const W*>(row + (int64_t)hh * D + L::piece(m, j)));
+            for (int j = 0; j < L::NC; ++j) {
+                const W* p = reinterpret_cast<const W*>(row + (int64_t)hh * D + L::piece(m, j));
+                w[i][j] = CACHED ? *p : __builtin_nontemporal_load(p);
+            }
         }
     }
     __device__ __forceinline__ void get(int i, float* f) const {
@@ -64,13 +66,14 @@ template <typename T, int D, int NG, int LPH> struct RowPieces {
 
 // Head layout as the forward's (HeadLanes): LPH lanes per head, NG groups of
 // 64 / LPH heads. SHORT (few rows): a block takes all rows of one group of heads
-// and writes the sums themselves, without a second launch.
-template <typename T, int D, int NG, int W, bool SHORT>
+// and writes the sums themselves, without a second launch. CACHED: row loads by
+// the default policy.
+template <typename T, int D, int NG, int W, bool SHORT, bool CACHED>
 __global__ __launch_bounds__(W * 64, SHORT ? 4 : sizeof(T) == 2 && NG < 4 ? 3 : 2) void qk_bwd_kernel(QkBwdArgs a, RopeSlots tab) {
     constexpr int LPH = (sizeof(T) == 2 && D == 64) ? 8 : 16;
     constexpr int HPI = 64 / LPH;
     using L = HeadLanes<T, D, LPH>;
-    using Pieces = RowPieces<T, D, NG, LPH>;
+    using Pieces = RowPieces<T, D, NG, LPH, CACHED>;
     constexpr int E = L::E, P = L::P, HALF = D / 2;
     // gamma * scale and bias while rows are worked on, the waves' sums afterwards
     __shared__ __attribute__((aligned(16))) float lds[W][NG * HPI * D];
@@ -330,9 +333,19 @@ int64_t blocks_for(int64_t rows, int tensors, int per_cu) {
 
 inline bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 
+// Rows of tensors that the 256 MB infinity cache holds in part are read through it;
+// above that the loads that pass it by are faster (q and k, 12 heads of 128, f16:
+// 302 MB in and out 65.4 -> 58.9 us, 453 MB 93.5 -> 92.0, 604 MB 122.5 -> 127.5; 4,096
+// rows of 16 heads of 64 18.5 -> 17.1). The stores always pass it by (the other way
+// 201,436 rows 683 -> 735 us).
+constexpr int64_t kCachedBytes = int64_t(400) << 20;
+
 template <typename T, int D, int NG>
 void launch_fast(const QkBwdArgs& a, const RopeSlots& tab, hipStream_t s) {
-    hipLaunchKernelGGL((qk_bwd_kernel<T, D, NG, kW, false>), dim3((unsigned)(a.blocks * a.tensors)), dim3(kW * 64), 0, s, a, tab);
+    const dim3 grid((unsigned)(a.blocks * a.tensors)), block(kW * 64);
+    if (3 * a.tensors * a.rows * a.heads * D * (int64_t)sizeof(T) <= kCachedBytes)
+        hipLaunchKernelGGL((qk_bwd_kernel<T, D, NG, kW, false, true>), grid, block, 0, s, a, tab);
+    else hipLaunchKernelGGL((qk_bwd_kernel<T, D, NG, kW, false, false>), grid, block, 0, s, a, tab);
 }
 
 template <typename T>
@@ -354,8 +367,8 @@ hipError_t launch_typed(const QkBwdArgs& a, const RopeSlots& tab, hipStream_t s)
         // 7.0 -> 8.8; eagerly every call saves another 2.5 us of launching
         const int hpi = sizeof(T) == 2 && a.head_dim == 64 ? 8 : 4;
         const dim3 grid((unsigned)((a.heads + hpi - 1) / hpi * a.tensors));
-        if (a.head_dim == 128) hipLaunchKernelGGL((qk_bwd_kernel<T, 128, 1, kShortW, true>), grid, dim3(kShortW * 64), 0, s, a, tab);
-        else hipLaunchKernelGGL((qk_bwd_kernel<T, 64, 1, kShortW, true>), grid, dim3(kShortW * 64), 0, s, a, tab);
+        if (a.head_dim == 128) hipLaunchKernelGGL((qk_bwd_kernel<T, 128, 1, kShortW, true, true>), grid, dim3(kShortW * 64), 0, s, a, tab);
+        else hipLaunchKernelGGL((qk_bwd_kernel<T, 64, 1, kShortW, true, true>), grid, dim3(kShortW * 64), 0, s, a, tab);
         return hipGetLastError();
     } else if (!fast) {
         const int64_t units = a.blocks * a.heads;
