@@ -68,26 +68,35 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnBwdArgs a) {
     }
     const T* x = q ? static_cast<const T*>(a.dout) + head * a.do_head : static_cast<const T*>(f.v) + head * f.v_head;
     const int64_t stride = q ? a.do_row : f.v_row;
+    // all rows' loads first: one wait for memory, not one a row
+    constexpr int kR = kPrepRows / 16;
     float most = 0.0f;
+    if (s.lo < s.hi) {
+        float v[kR][E], o[kR][E], lse[kR];
 #pragma unroll
-    for (int i = 0; i < kPrepRows / 16; ++i) {
-        const int row = s.lo + i * 16 + rr;
-        if (row >= s.hi) break;
-        float v[E];
-        load_elems<T, E>(x + row * stride + m * E, v);
-        if (kF16) most = fmaxf(most, row16_sum(sum_sq_all<E>(v)));
-        if (q) {
-            float o[E], d = 0.0f;
-            load_elems<T, E>(static_cast<const T*>(f.out) + row * f.o_row + head * f.o_head + m * E, o);
+        for (int i = 0; i < kR; ++i) {
+            const int at = s.lo + i * 16 + rr, row = at < s.hi ? at : s.hi - 1;
+            load_elems<T, E>(x + row * stride + m * E, v[i]);
+            if (q) {
+                load_elems<T, E>(static_cast<const T*>(f.out) + row * f.o_row + head * f.o_head + m * E, o[i]);
+                lse[i] = f.lse[head * f.q_rows + row];
+            }
+        }
 #pragma unroll
-            for (int e = 0; e < E; ++e) d = fmaf(v[e], o[e], d);
-            d = row16_sum(d);
-            if (m == 0) {
-                const int64_t at = head * f.q_rows + row;
-                const float lse = f.lse[at];
-                a.delta[at] = d;
-                // a row without keys: P = 0
-                a.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e - (kF16 ? kShiftP : 0.0f);
+        for (int i = 0; i < kR; ++i) {
+            const int row = s.lo + i * 16 + rr;
+            if (kF16) most = fmaxf(most, row16_sum(sum_sq_all<E>(v[i])));   // (a clamped row's counts anyway)
+            if (q) {
+                float d = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) d = fmaf(v[i][e], o[i][e], d);
+                d = row16_sum(d);
+                if (m == 0 && row < s.hi) {
+                    const int64_t at = head * f.q_rows + row;
+                    a.delta[at] = d;
+                    // a row without keys: P = 0
+                    a.lse2[at] = lse[i] == -INFINITY ? INFINITY : lse[i] * kLog2e - (kF16 ? kShiftP : 0.0f);
+                }
             }
         }
     }
