@@ -383,13 +383,20 @@ enum Form { kLarge, kSmall, kFew };
 // Large: where its blocks fill 1.5 places a CU; below, the small form's twice as
 // many blocks do better (2,368 queries, 1,029 keys, 16 heads of 64: small 23.6 us,
 // large 26.9; 8,192 queries, 12 heads of 128: 73 and 62), and for segments within
-// its tile (64 of 37 tokens: 6.9 and 9.5).
+// its tile (64 of 37 tokens: 6.9 and 9.5). With heads of 64 a CU holds four small
+// blocks, and its time goes by their number: a small block counts 5, a large one 9
+// (4,096 tokens: 12 heads, 3 small or 2 large, 66.3 and 74.6 us; 16, 4 or 2, 85.8 and
+// 79.1; 20, 5 or 3, 108 and 115; 24, 6 or 3, 126 and 117). With heads of 128 it holds
+// two of either (12 heads 120 and 113).
 
 Form form_of(const AttnArgs& a) {
     const int64_t rows = (a.q_rows + a.nbatch - 1) / a.nbatch, cu = device_cu_count();
     if (rows <= 16) return kFew;
-    const int64_t per = (int64_t)a.nbatch * a.heads;
-    return (rows + 127) / 128 * per * 2 < cu * 3 || rows <= 64 ? kSmall : kLarge;
+    const int64_t per = (int64_t)a.nbatch * a.heads, large = (rows + 127) / 128 * per;
+    if (large * 2 < cu * 3 || rows <= 64) return kSmall;
+    const auto each = [cu](int64_t blocks) { return (blocks + cu - 1) / cu; };   // blocks on the fullest CU
+    if (a.head_dim == 64 && each((rows + 63) / 64 * per) * 5 < each(large) * 9) return kSmall;
+    return kLarge;
 }
 
 template <typename T, int D, typename F, bool SPLIT>
