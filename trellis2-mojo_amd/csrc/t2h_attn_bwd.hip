@@ -567,7 +567,7 @@ constexpr int kSplitRows = 1024;                   // streaming tokens that a pa
 // results a few terms of a sum weigh most, whose rounding does not average out
 // (one query, 10,474 keys, f16: dk is 3.4e-4 off in the 2-norm, and so as little
 // as its own rounding, 2.2e-4; 16 queries, 60,000 keys 323 -> 381 us).
-struct Plan { bool small; int split; int64_t blocks; };   // blocks: of the small form, unsplit
+struct Plan { bool small; int split; int64_t blocks; };   // blocks: unsplit
 Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads, bool fine) {
     const int64_t cu = device_cu_count(), per = (int64_t)nbatch * heads;
     const int64_t large = ((int64_t)kept.share + kRowsLarge - 1) / kRowsLarge * per;
@@ -584,21 +584,29 @@ Plan plan_of(const AttnSide& kept, int64_t stream, int32_t nbatch, int32_t heads
         if (n > most) n = most;
     }
     p.split = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-    p.blocks = small;
+    p.blocks = p.small ? small : large;
     return p;
 }
-// Parts for both sides' small blocks at once; a block of dk, dv does 4 products
-// a streaming token, one of dq 3.
+// Parts for both sides at once, where both have the same form; a block of dk, dv
+// does 4 products a streaming token, one of dq 3. Large blocks that fill the GPU's
+// places together stay whole on a side where one is no longer than a place's share
+// (2,048 tokens, 16 heads of 64, 512 blocks: each side in 2 parts 88 us, whole 71).
 void share_cus(Plan& q, int64_t keys, Plan& kv, int64_t queries) {
-    const int64_t cu = device_cu_count();
-    if (!q.small || !kv.small || q.blocks + kv.blocks > cu) return;
-    const int64_t each = (q.blocks * keys * 3 + kv.blocks * queries * 4) / (cu * 4), len = each > 256 ? each : 256;
-    const auto parts = [len](int64_t stream) {
-        const int64_t n = (stream + len / 2) / len;
-        return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-    };
-    q.split = parts(keys);
-    kv.split = parts(queries);
+    const int64_t cu = device_cu_count(), blocks = q.blocks + kv.blocks;
+    const int64_t work = q.blocks * keys * 3 + kv.blocks * queries * 4;
+    if (q.small && kv.small && blocks <= cu) {
+        const int64_t each = work / (cu * 4), len = each > 256 ? each : 256;
+        const auto parts = [len](int64_t stream) {
+            const int64_t n = (stream + len / 2) / len;
+            return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+        };
+        q.split = parts(keys);
+        kv.split = parts(queries);
+    } else if (!q.small && !kv.small && blocks >= 2 * cu) {
+        const int64_t share = work / (2 * cu);
+        if (keys * 12 <= share * 5) q.split = 1;
+        if (queries * 16 <= share * 5) kv.split = 1;
+    }
 }
 
 template <typename T, int D, int KV, int Q>
