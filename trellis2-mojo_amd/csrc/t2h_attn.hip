@@ -291,21 +291,20 @@ __global__ __launch_bounds__(NW * KG * 64, 2) void attn_kernel(AttnArgs a) {
     }
 }
 
-// Join of the splits: out = sum_s exp2(lse_s - lse) out_s. A wave takes STRANDS
-// splits at a time of 4 / STRANDS (row, head)s, 16 lanes each, D / 16 elements a
-// lane; WAVES waves share a (row, head)'s splits and meet in LDS. Up to 8 splits
-// (many rows) one strand each; more would be a chain of as many loads, and go to 16
-// strands (whole calls: 1,000 queries in 4 splits one strand 17.0 us, 16 20.3; one
-// query in 16 splits 13.2 and 9.6, in 64 42 and 24).
-template <typename T, int D, int STRANDS, int WAVES>
+// Join of the splits: out = sum_s exp2(lse_s - lse) out_s. 16 lanes take a (row,
+// head), D / 16 elements a lane, and its splits in turn; MANY: a block's 16 such
+// strands share the splits of one (row, head), and meet in LDS. Up to 8 splits (many
+// rows) one strand each; more would be a chain of as many loads (whole calls: 1,000
+// queries in 4 splits one strand 17.0 us, 16 20.3; one query in 16 splits 13.2 and
+// 9.6, in 64 42 and 24).
+template <typename T, int D, bool MANY>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    constexpr int E = D / 16, kUnits = 16 / (STRANDS * WAVES);
-    static_assert(STRANDS == 1 || STRANDS == 4, "lanes");
+    constexpr int E = D / 16, kWaves = 4;
     const int wave = threadIdx.x >> 6, lane = lane_id(), m = lane & 15, h = lane >> 4;
     const int64_t total = a.q_rows * a.heads;
-    const int64_t u0 = block_linear() * kUnits + (STRANDS == 1 ? (WAVES == 1 ? wave * 4 + h : h) : (WAVES == 1 ? wave : 0));
+    const int strand = wave * 4 + h, first = MANY ? strand : 0;
+    const int64_t u0 = MANY ? block_linear() : block_linear() * 16 + strand;
     const int64_t u = u0 < total ? u0 : total - 1;
-    const int first = STRANDS == 1 ? (WAVES == 1 ? 0 : wave) : (WAVES == 1 ? h : wave * 4 + h);
     const int64_t row = u / a.heads;
     const int head = (int)(u - row * a.heads);
     const float* pl = a.part_lse + head * a.q_rows + row;
@@ -313,7 +312,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int64_t ls = a.heads * a.q_rows, os = ls * D;
     float top = -INFINITY, sum = 0.0f, acc[E] = {};
 #pragma unroll 4
-    for (int s = first; s < a.nsplit; s += STRANDS * WAVES) {
+    for (int s = first; s < a.nsplit; s += MANY ? 16 : 1) {
         const float l = pl[s * ls];
         float v[E];
         load_params<E>(po + s * os, v);
@@ -332,7 +331,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + v[e] * w1;
     };
-    if constexpr (STRANDS == 4) {
+    if constexpr (MANY) {
 #pragma unroll
         for (int x = 16; x < 64; x <<= 1) {
             const float t1 = __shfl_xor(top, x), s1 = __shfl_xor(sum, x);
@@ -341,9 +340,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
             for (int e = 0; e < E; ++e) v[e] = __shfl_xor(acc[e], x);
             join(t1, s1, v);
         }
-    }
-    if constexpr (WAVES > 1) {
-        __shared__ float lt[WAVES][16], lm[WAVES][16], lo[WAVES][16][E];
+        __shared__ float lt[kWaves][16], lm[kWaves][16], lo[kWaves][16][E];
         if (h == 0) {
             lt[wave][m] = top;
             lm[wave][m] = sum;
@@ -352,14 +349,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
         }
         __syncthreads();
         if (wave > 0) return;
-        for (int w = 1; w < WAVES; ++w) {
+        for (int w = 1; w < kWaves; ++w) {
             float v[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = lo[w][m][e];
             join(lt[w][m], lm[w][m], v);
         }
     }
-    if (u0 >= total || (STRANDS == 4 && h > 0)) return;
+    if (u0 >= total || (MANY && h > 0)) return;
     if (a.qs.offsets != nullptr && (row < a.qs.offsets[0] || row >= a.qs.offsets[a.nbatch])) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -416,8 +413,8 @@ hipError_t launch_d(AttnArgs a, hipStream_t s) {
     }
     if (a.nsplit > 1) {
         const int64_t units = a.q_rows * a.heads;
-        if (a.nsplit > 8) hipLaunchKernelGGL((attn_join_kernel<T, D, 4, 4>), grid_1d(units), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((attn_join_kernel<T, D, 1, 1>), grid_1d((units + 15) / 16), dim3(256), 0, s, a);
+        if (a.nsplit > 8) hipLaunchKernelGGL((attn_join_kernel<T, D, true>), grid_1d(units), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((attn_join_kernel<T, D, false>), grid_1d((units + 15) / 16), dim3(256), 0, s, a);
     }
     return hipGetLastError();
 }
